@@ -1,0 +1,284 @@
+// Rotary position embedding with several position axes (time, height, width
+// of images and video) for gfx950.
+//
+// Pair i < D/2 of a head turns by the angle of ONE axis a(i):
+//   P = positions[a(i), b, t],  c = cos[P, i],  s = sin[P, i]
+//   y[i]       = x[i] c - x[i + D/2] s
+//   y[i + D/2] = x[i + D/2] c + x[i] s
+// a(i) is given by sections n_0 .. n_{A-1} (sum D/2): either runs of n_a
+// pairs, or interleaved (a = i mod A while i < A n_a, else axis 0). The
+// backward is the same map with -s. Arithmetic is fp32, rounded once.
+//
+// HBM-bound: every element of q and k is read and written once, 3 flops an
+// element. cos/sin rows are gathered from the table, which caches hold (a row
+// is read by every head of its token). So a lane keeps the cos/sin of its VEC
+// pairs of one token in registers and walks over heads with them: a chain of
+// position load -> table load once, then streaming. Consecutive lanes cover
+// the chunks of a head, then heads of the token ([B, T, H, D] storage) or
+// tokens of the head ([B, H, T, D] storage), so that a wave touches one
+// contiguous span either way.
+//
+// A position outside [0, table rows) reads nothing and gives NaN in the pairs
+// of its axis.
+#include "hk_common.h"
+#include "../../include/hilda_kernel_amd.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace hk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxAxes = 4;
+
+struct Axes {
+  int count;
+  int interleaved;
+  int n[kMaxAxes];  // sections; runs: n[a] = first pair past axis a
+};
+
+struct Heads {
+  int count;
+  int64_t is_b, is_h, is_t;  // element strides of the input
+  int64_t os_b, os_h, os_t;  // and of the output
+};
+
+struct RopeAxesArgs {
+  Heads q, k;
+  const void* positions;
+  int64_t ps_a, ps_b, ps_t;
+  int64_t table_rows, table_ld;
+  Axes axes;
+  uint32_t T, half;
+  uint32_t chunks;       // half / VEC
+  uint32_t lanes;        // lanes of one head: min(chunks, 256)
+  uint32_t slots;        // a lane walks heads slot, slot + slots, ...
+  uint32_t tokens_block; // tokens a block covers
+  uint32_t blocks_row;   // [B, H, T, D] order: blocks per (batch, slot)
+  int64_t tokens;        // B * T
+  float sgn;
+};
+
+__device__ __forceinline__ int axis_of(const Axes& ax, int pair) {
+  if (ax.interleaved) {
+    int a = pair % ax.count;
+    int n = ax.n[0];
+#pragma unroll
+    for (int j = 1; j < kMaxAxes; ++j) n = a == j ? ax.n[j] : n;
+    return pair < ax.count * n ? a : 0;
+  }
+  int a = 0;
+#pragma unroll
+  for (int j = 0; j < kMaxAxes - 1; ++j) a += (j < ax.count - 1 && pair >= ax.n[j]) ? 1 : 0;
+  return a;
+}
+
+template <typename T, typename C, typename P, int VEC, bool HEAD_MAJOR>
+__global__ __launch_bounds__(kThreads) void rope_axes_kernel(T* __restrict__ q_out, const T* __restrict__ q_in,
+                                                             T* __restrict__ k_out, const T* __restrict__ k_in,
+                                                             const C* __restrict__ cosp, const C* __restrict__ sinp,
+                                                             RopeAxesArgs g) {
+  const uint32_t lane_c = threadIdx.x % g.lanes;
+  const uint32_t rest = threadIdx.x / g.lanes;
+  const uint32_t chunk = blockIdx.y * g.lanes + lane_c;
+  int64_t b;
+  uint32_t t, slot;
+  if constexpr (HEAD_MAJOR) {
+    const uint32_t group = blockIdx.x / g.blocks_row;
+    t = (blockIdx.x % g.blocks_row) * g.tokens_block + rest;
+    slot = group % g.slots;
+    b = group / g.slots;
+    if (rest >= g.tokens_block || t >= g.T || chunk >= g.chunks) return;
+  } else {
+    const uint32_t local = rest / g.slots;
+    slot = rest % g.slots;
+    const int64_t n = (int64_t)blockIdx.x * g.tokens_block + local;
+    if (local >= g.tokens_block || n >= g.tokens || chunk >= g.chunks) return;
+    b = (uint32_t)n / g.T;
+    t = (uint32_t)n % g.T;
+  }
+  const int first = (int)chunk * VEC;
+
+  // cos/sin of this lane's pairs, an axis at a time
+  float c[VEC], s[VEC];
+  int axis[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) axis[i] = axis_of(g.axes, first + i);
+  const P* pos = static_cast<const P*>(g.positions) + b * g.ps_b + t * g.ps_t;
+#pragma unroll
+  for (int a = 0; a < kMaxAxes; ++a) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) any = any || axis[i] == a;
+    if (a < g.axes.count && any) {
+      const int64_t at = (int64_t)pos[a * g.ps_a];
+      const bool in = at >= 0 && at < g.table_rows;
+      float ca[VEC], sa[VEC];
+      if (in) {
+        unpack(load_pack<C, VEC>(cosp + at * g.table_ld + first), ca);
+        unpack(load_pack<C, VEC>(sinp + at * g.table_ld + first), sa);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if (axis[i] == a) {
+          c[i] = in ? ca[i] : __builtin_nanf("");
+          s[i] = in ? sa[i] * g.sgn : __builtin_nanf("");
+        }
+      }
+    }
+  }
+
+  const int heads = g.q.count + g.k.count;
+  for (int h = (int)slot; h < heads; h += (int)g.slots) {
+    const bool is_q = h < g.q.count;
+    const int hh = is_q ? h : h - g.q.count;
+    const T* in = (is_q ? q_in : k_in) + b * (is_q ? g.q.is_b : g.k.is_b) + hh * (is_q ? g.q.is_h : g.k.is_h) +
+                  t * (is_q ? g.q.is_t : g.k.is_t) + first;
+    T* out = (is_q ? q_out : k_out) + b * (is_q ? g.q.os_b : g.k.os_b) + hh * (is_q ? g.q.os_h : g.k.os_h) +
+             t * (is_q ? g.q.os_t : g.k.os_t) + first;
+    float x1[VEC], x2[VEC], y1[VEC], y2[VEC];
+    unpack(load_pack<T, VEC>(in), x1);
+    unpack(load_pack<T, VEC>(in + g.half), x2);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      y1[i] = x1[i] * c[i] - x2[i] * s[i];
+      y2[i] = x2[i] * c[i] + x1[i] * s[i];
+    }
+    store_pack<T, VEC>(out, pack<T, VEC>(y1));
+    store_pack<T, VEC>(out + g.half, pack<T, VEC>(y2));
+  }
+}
+
+template <typename T> struct Tag { using type = T; };
+
+template <typename F>
+int dispatch_t(int dt, F&& f) {
+  switch (dt) {
+    case kF32: return f(Tag<float>{});
+    case kF16: return f(Tag<_Float16>{});
+    case kBF16: return f(Tag<__bf16>{});
+  }
+  set_error("invalid dtype code %d", dt);
+  return HK_EINVAL;
+}
+
+bool heads_ok(const Heads& h, const void* in, const void* out, int vec, int es) {
+  const int64_t s[6] = {h.is_b, h.is_h, h.is_t, h.os_b, h.os_h, h.os_t};
+  for (const int64_t v : s)
+    if (v % vec) return false;
+  return h.count == 0 || (aligned_to(in, (size_t)vec * es) && aligned_to(out, (size_t)vec * es));
+}
+
+}  // namespace
+}  // namespace hk
+
+using namespace hk;
+
+extern "C" {
+
+int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int64_t q_in_sH, int64_t q_in_sT,
+                 int64_t q_out_sB, int64_t q_out_sH, int64_t q_out_sT, void* k_out, const void* k_in, int64_t Hk,
+                 int64_t k_in_sB, int64_t k_in_sH, int64_t k_in_sT, int64_t k_out_sB, int64_t k_out_sH,
+                 int64_t k_out_sT, const void* cos, const void* sin, int64_t table_rows, int64_t table_ld,
+                 const void* positions, int pos_type, int64_t pos_sA, int64_t pos_sB, int64_t pos_sT,
+                 const int64_t* sections, int axes, int interleaved, int64_t B, int64_t T, int64_t D, int dtype_x,
+                 int dtype_cs, int inverse, hk_stream_t stream) {
+  HK_REQUIRE(B >= 0 && T >= 0 && Hq >= 0 && Hk >= 0 && D > 0, "invalid shape B=%lld T=%lld Hq=%lld Hk=%lld D=%lld",
+             (long long)B, (long long)T, (long long)Hq, (long long)Hk, (long long)D);
+  HK_REQUIRE(D % 2 == 0, "head_dim D=%lld must be even", (long long)D);
+  HK_REQUIRE(dtype_cs == kF32 || dtype_cs == kF16 || dtype_cs == kBF16, "invalid cos/sin dtype %d", dtype_cs);
+  HK_REQUIRE(dtype_x == kF32 || dtype_x == kF16 || dtype_x == kBF16, "invalid dtype code %d", dtype_x);
+  HK_REQUIRE(pos_type == HK_I32 || pos_type == HK_I64, "positions must be int32 or int64, got code %d", pos_type);
+  HK_REQUIRE(axes >= 1 && axes <= kMaxAxes, "1..%d position axes, got %d", kMaxAxes, axes);
+  HK_REQUIRE(sections != nullptr, "null pointer argument");
+  const int64_t half = D / 2;
+  RopeAxesArgs g = {};
+  int64_t sum = 0;
+  for (int a = 0; a < axes; ++a) {
+    HK_REQUIRE(sections[a] >= 0, "sections must not be negative");
+    sum += sections[a];
+    g.axes.n[a] = (int)(interleaved ? sections[a] : sum);
+  }
+  HK_REQUIRE(sum == half, "sections sum to %lld, need D/2 = %lld", (long long)sum, (long long)half);
+  if (interleaved) {
+    // axis a > 0 owns pairs a, a + A, ..., a + A (n_a - 1); all of them must exist
+    for (int a = 1; a < axes; ++a)
+      HK_REQUIRE(sections[a] == 0 || a + axes * (sections[a] - 1) < half,
+                 "interleaved section %d of %lld pairs does not fit D/2 = %lld", a, (long long)sections[a],
+                 (long long)half);
+  }
+  g.axes.count = axes;
+  g.axes.interleaved = interleaved ? 1 : 0;
+  const int64_t strides[] = {q_in_sB,  q_in_sH,  q_in_sT,  q_out_sB, q_out_sH, q_out_sT, k_in_sB, k_in_sH, k_in_sT,
+                             k_out_sB, k_out_sH, k_out_sT, pos_sA,   pos_sB,   pos_sT};
+  for (const int64_t s : strides) HK_REQUIRE(s >= 0, "negative strides are not supported");
+  HK_REQUIRE(table_rows >= 0 && table_ld >= half, "cos/sin row stride %lld smaller than D/2 = %lld",
+             (long long)table_ld, (long long)half);
+  HK_REQUIRE(B == 0 || T <= ((1LL << 31) - 1) / B, "B * T = %lld * %lld too large", (long long)B, (long long)T);
+  HK_REQUIRE(Hq + Hk < (1 << 20) && D <= (1 << 20), "too many heads or too long a head");
+  if (B == 0 || T == 0 || Hq + Hk == 0) return HK_OK;
+  HK_REQUIRE((Hq == 0 || (q_out && q_in)) && (Hk == 0 || (k_out && k_in)) && cos && sin && positions,
+             "null pointer argument");
+  g.q = {(int)Hq, q_in_sB, q_in_sH, q_in_sT, q_out_sB, q_out_sH, q_out_sT};
+  g.k = {(int)Hk, k_in_sB, k_in_sH, k_in_sT, k_out_sB, k_out_sH, k_out_sT};
+  g.positions = positions;
+  g.ps_a = pos_sA;
+  g.ps_b = pos_sB;
+  g.ps_t = pos_sT;
+  g.table_rows = table_rows;
+  g.table_ld = table_ld;
+  g.T = (uint32_t)T;
+  g.half = (uint32_t)half;
+  g.tokens = B * T;
+  g.sgn = inverse ? -1.f : 1.f;
+  // the storage order of the larger tensor decides how lanes walk memory
+  const Heads& lead = Hq >= Hk ? g.q : g.k;
+  const bool head_major = T > 1 && lead.is_t < lead.is_h;
+  const hipStream_t st = (hipStream_t)stream;
+
+  return dispatch_t(dtype_x, [&](auto tx) {
+    using TX = typename decltype(tx)::type;
+    return dispatch_t(dtype_cs, [&](auto tc) {
+      using TC = typename decltype(tc)::type;
+      auto launch = [&](auto vec_c) {
+        constexpr int VEC = decltype(vec_c)::value;
+        g.chunks = (uint32_t)(half / VEC);
+        g.lanes = std::min<uint32_t>(g.chunks, kThreads);
+        const uint32_t per_block = kThreads / g.lanes;
+        const int64_t heads = Hq + Hk;
+        g.slots = (uint32_t)std::min<int64_t>(heads, head_major ? heads : per_block);
+        dim3 grid(1, (unsigned)cdiv((int64_t)g.chunks, (int64_t)g.lanes));
+        int64_t blocks;
+        if (head_major) {
+          g.tokens_block = per_block;
+          g.blocks_row = (uint32_t)cdiv(T, (int64_t)per_block);
+          blocks = B * (int64_t)g.slots * g.blocks_row;
+        } else {
+          g.tokens_block = per_block / g.slots;
+          blocks = cdiv(g.tokens, (int64_t)g.tokens_block);
+        }
+        HK_REQUIRE(blocks < (1LL << 31), "too many rows for one launch");
+        grid.x = (unsigned)blocks;
+        auto go = [&](auto tp, auto order) {
+          using TP = typename decltype(tp)::type;
+          constexpr bool HM = decltype(order)::value;
+          hipLaunchKernelGGL((rope_axes_kernel<TX, TC, TP, VEC, HM>), grid, dim3(kThreads), 0, st, (TX*)q_out,
+                             (const TX*)q_in, (TX*)k_out, (const TX*)k_in, (const TC*)cos, (const TC*)sin, g);
+          return check_launch("rope_axes_kernel");
+        };
+        if (pos_type == HK_I64)
+          return head_major ? go(Tag<int64_t>{}, std::true_type{}) : go(Tag<int64_t>{}, std::false_type{});
+        return head_major ? go(Tag<int32_t>{}, std::true_type{}) : go(Tag<int32_t>{}, std::false_type{});
+      };
+      constexpr int V = 16 / sizeof(TX);
+      const bool whole = half % V == 0 && heads_ok(g.q, q_in, q_out, V, sizeof(TX)) &&
+                         heads_ok(g.k, k_in, k_out, V, sizeof(TX)) && table_ld % V == 0 &&
+                         aligned_to(cos, sizeof(TC) * V) && aligned_to(sin, sizeof(TC) * V);
+      if (whole) return launch(std::integral_constant<int, V>{});
+      return launch(std::integral_constant<int, 1>{});
+    });
+  });
+}
+
+}  // extern "C"

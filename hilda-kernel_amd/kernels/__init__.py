@@ -11,6 +11,8 @@ with the reference.
 """
 from .rms_norm import HildaRMSNormFunction, hilda_rms_norm, RMSNorm
 from .rope import HildaRopeFunction, hilda_rope, RotaryEmbedding
+from .rope_axes import HildaRopeAxesFunction, hilda_rope_axes, MultiAxisRotaryEmbedding
+from .rms_norm_quant import (hilda_rms_norm_quant, RMSNormQuant, hilda_fused_add_rms_norm_quant, FusedAddRMSNormQuant)
 from .swiglu import HildaSwiGLUFunction, hilda_swiglu, SwiGLU
 from .geglu import HildaGeGLUFunction, hilda_geglu, GeGLU
 from .kl_div import HildaKLDivFunction, hilda_kl_div, KLDivLoss
@@ -22,11 +24,14 @@ from .fused_add_rms_norm import HildaFusedAddRMSNormFunction, hilda_fused_add_rm
 from .fused_linear_cross_entropy import (HildaFusedLinearCrossEntropyFunction, hilda_fused_linear_cross_entropy,
                                          FusedLinearCrossEntropyLoss)
 from .grpo_loss import HildaGRPOLossFunction, hilda_grpo_loss, GRPOLoss, fused_selective_log_softmax
+from .sampling import hilda_sample
 from .fused_linear_grpo import HildaFusedLinearGRPOFunction, hilda_fused_linear_grpo_loss, FusedLinearGRPOLoss
 
 __all__ = [
     "HildaRMSNormFunction", "hilda_rms_norm", "RMSNorm",
     "HildaRopeFunction", "hilda_rope", "RotaryEmbedding",
+    "HildaRopeAxesFunction", "hilda_rope_axes", "MultiAxisRotaryEmbedding",
+    "hilda_rms_norm_quant", "RMSNormQuant", "hilda_fused_add_rms_norm_quant", "FusedAddRMSNormQuant",
     "HildaSwiGLUFunction", "hilda_swiglu", "SwiGLU",
     "HildaGeGLUFunction", "hilda_geglu", "GeGLU",
     "HildaKLDivFunction", "hilda_kl_div", "KLDivLoss",
@@ -37,5 +42,6 @@ __all__ = [
     "HildaFusedAddRMSNormFunction", "hilda_fused_add_rms_norm", "FusedAddRMSNorm",
     "HildaFusedLinearCrossEntropyFunction", "hilda_fused_linear_cross_entropy", "FusedLinearCrossEntropyLoss",
     "HildaGRPOLossFunction", "hilda_grpo_loss", "GRPOLoss", "fused_selective_log_softmax",
+    "hilda_sample",
     "HildaFusedLinearGRPOFunction", "hilda_fused_linear_grpo_loss", "FusedLinearGRPOLoss",
 ]

@@ -25,6 +25,7 @@ _MASK_CODE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torc
               torch.int32: I32, torch.int64: I64}
 
 _i32, _i64, _f32, _p, _sz = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/hilda_kernel_amd.h
 SIGNATURES = {
@@ -42,6 +43,10 @@ SIGNATURES = {
     "hk_rope": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                        _i32, _i32, _i32, _p]),
     "hk_rope_qk": (_i32, [_p, _p] + [_i64] * 7 + [_p, _p] + [_i64] * 7 + [_p, _p] + [_i64] * 6 + [_i32, _i32, _i32, _p]),
+    "hk_rope_axes": (_i32, [_p, _p] + [_i64] * 7 + [_p, _p] + [_i64] * 7 + [_p, _p, _i64, _i64, _p, _i32, _i64, _i64, _i64,
+                            _p, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _p]),
+    "hk_rms_norm_quant_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _i32, _f32, _p]),
+    "hk_sample": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _p, _f64, _p, _i32, _i64, _p, _f64, _p, _f64, _i32, _p]),
     "hk_swiglu_fwd": (_i32, [_p, _p, _p, _i64, _i32, _p]),
     "hk_swiglu_bwd": (_i32, [_p, _p, _p, _p, _p, _i64, _i32, _p]),
     "hk_geglu_fwd": (_i32, [_p, _p, _p, _i64, _i32, _p]),
@@ -120,6 +125,15 @@ def call(name: str, *args) -> None:
     status = getattr(_lib or load(), name)(*args)
     if status:
         check(status, name)
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """``call`` with the device's current stream as the last argument, that device being made current for the launch."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        call(name, *args, stream_of(device))
+        return
+    with torch.cuda.device(device):
+        call(name, *args, stream_of(device))
 
 
 def dtype_code(t: torch.Tensor) -> int:

@@ -115,6 +115,17 @@ int hk_fused_add_rms_norm_bwd(void* dx, void* dw, const void* dy, const void* ds
                               int dtype_x, int dtype_w, int dw_mode, void* workspace, size_t workspace_bytes,
                               hk_stream_t stream);
 
+/* RMSNorm with an e4m3 output and fp32 scales (no counterpart in the
+ * reference, whose norms are unquantised): y = RMSNorm(s) * w, s = x + r
+ * rounded to dtype_x and stored (r and s NULL: s = x); per row (group 0) or
+ * group of 32, 64, 128 or 256 columns, scale = max(max|y| / 448, 2^-100) and
+ * q = e4m3(y / scale). q, s [rows, cols] and scale [rows, 1 or cols / group]
+ * are contiguous, x and r have row stride ld; rstd (nullable) as of
+ * hk_rms_norm_fwd, for the unquantised norms' backward. */
+int hk_rms_norm_quant_fwd(void* q, float* scale, void* s, float* rstd, const void* x, const void* r, const void* w,
+                          int64_t rows, int64_t cols, int64_t ld, int64_t group, int dtype_x, int dtype_w, float eps,
+                          hk_stream_t stream);
+
 /* ----------------------------------------------------------------------- */
 /* RoPE                                                                    */
 /* ----------------------------------------------------------------------- */
@@ -138,6 +149,24 @@ int hk_rope_qk(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int64
                int64_t k_in_sB, int64_t k_in_sH, int64_t k_in_sT, int64_t k_out_sB, int64_t k_out_sH,
                int64_t k_out_sT, const void* cos, const void* sin, int64_t B, int64_t T, int64_t D, int64_t cos_B,
                int64_t cos_sB, int64_t cos_sT, int dtype_x, int dtype_cs, int inverse, hk_stream_t stream);
+
+/* Multi-axis RoPE (no counterpart in the reference, whose tokens sit at the
+ * positions 0..T-1 of one axis, rope.py:113-136): q (B, Hq, T, D) and
+ * k (B, Hk, T, D) in one launch, strides as for hk_rope_qk. Pair i < D/2 turns
+ * by row positions[a(i), b, t] of the cos/sin tables [table_rows, D/2] (last
+ * dim contiguous, row stride table_ld), a(i) the axis that `sections` (host
+ * array of `axes` counts, 1..4, sum D/2) gives it: runs of sections[a] pairs,
+ * or with `interleaved` a = i mod axes while i < axes * sections[a], else 0.
+ * positions: HK_I32 or HK_I64, element strides per axis, batch and token. A
+ * position outside [0, table_rows) gives NaN in its axis' pairs. inverse = 1
+ * rotates back (the backward). out must not overlap in. */
+int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int64_t q_in_sH, int64_t q_in_sT,
+                 int64_t q_out_sB, int64_t q_out_sH, int64_t q_out_sT, void* k_out, const void* k_in, int64_t Hk,
+                 int64_t k_in_sB, int64_t k_in_sH, int64_t k_in_sT, int64_t k_out_sB, int64_t k_out_sH,
+                 int64_t k_out_sT, const void* cos, const void* sin, int64_t table_rows, int64_t table_ld,
+                 const void* positions, int pos_type, int64_t pos_sA, int64_t pos_sB, int64_t pos_sT,
+                 const int64_t* sections, int axes, int interleaved, int64_t B, int64_t T, int64_t D, int dtype_x,
+                 int dtype_cs, int inverse, hk_stream_t stream);
 
 /* ----------------------------------------------------------------------- */
 /* SwiGLU                                                                  */
@@ -345,6 +374,23 @@ int hk_scale_rows(void* out, const void* in, const float* g, const float* g_prev
 int hk_selective_log_softmax(float* logp, const void* logits, const int64_t* ids, int64_t ids_sB, int64_t ids_sL,
                              const void* mask, int mask_dtype, int64_t mask_sB, int64_t mask_sL, int64_t B, int64_t L,
                              int64_t V, float temperature, int dtype, hk_stream_t stream);
+
+/* Token sampling (no counterpart in the reference, which scores completions
+ * but draws none): per row of logits [rows, cols] (row stride ld), z = x / T
+ * and the order x descending, lower index first among ties: the first top_k
+ * (<= 0 or >= cols: all), of those the shortest prefix with mass >= top_p of
+ * theirs (>= 1: all), of those the ones with e^(z - max) >= min_p. ids[row] is
+ * the first kept index with running mass > u[row] * total (index order; the
+ * last one with mass if none), logp[row] = z_id - log sum_j e^(z_j) over all
+ * cols. Each setting is one value, or fp32 (top_k: HK_I32 or HK_I64) values
+ * of the rows when its pointer is not NULL. A row with a NaN, a +inf or
+ * nothing above -inf, or with T outside [2^-64, 2^64], u outside [0, 1] or a
+ * NaN setting, gives id -1 and logp NaN; row values of top_p below 0 or of
+ * min_p above 1 count as 0 and 1. */
+int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int64_t rows, int64_t cols, int64_t ld,
+              const float* temperature_rows, double temperature, const void* top_k_rows, int top_k_type, int64_t top_k,
+              const float* top_p_rows, double top_p, const float* min_p_rows, double min_p, int dtype,
+              hk_stream_t stream);
 
 /* Bytes of device workspace hk_grpo_loss_fwd needs. */
 size_t hk_grpo_workspace_size(int64_t B, int64_t L);
