@@ -10,13 +10,17 @@
 // backward is the same map with -s. Arithmetic is fp32, rounded once.
 //
 // HBM-bound: every element of q and k is read and written once, 3 flops an
-// element. cos/sin rows are gathered from the table, which caches hold (a row
-// is read by every head of its token). So a lane keeps the cos/sin of its VEC
-// pairs of one token in registers and walks over heads with them: a chain of
-// position load -> table load once, then streaming. Consecutive lanes cover
-// the chunks of a head, then heads of the token ([B, T, H, D] storage) or
-// tokens of the head ([B, H, T, D] storage), so that a wave touches one
-// contiguous span either way.
+// element. A block takes a few tokens with all their heads: its threads gather
+// the tokens' (cos, sin) into LDS, one pair each (position, then table entry;
+// caches hold both), while the loads of their first heads are in flight; then a
+// lane walks over heads with the cos/sin of its VEC pairs in registers. With
+// the angles fetched by every lane for itself, 8 pairs of up to 3 axes each,
+// the selects alone took as long as the copy (53 us instead of 31.4 for q and k
+// of 8192 tokens x 40 heads x 128 bf16, 168 MB; a copy of them 30.2).
+// Consecutive lanes cover the chunks of a head, then heads of the token
+// ([B, T, H, D] storage) or tokens of the head ([B, H, T, D] storage), so that
+// a wave touches one contiguous span either way. Stores are non-temporal (1 us
+// of the 31.4).
 //
 // A position outside [0, table rows) reads nothing and gives NaN in the pairs
 // of its axis.
@@ -55,7 +59,6 @@ struct RopeAxesArgs {
   uint32_t lanes;        // lanes of one head: min(chunks, 256)
   uint32_t slots;        // a lane walks heads slot, slot + slots, ...
   uint32_t tokens_block; // tokens a block covers
-  uint32_t blocks_row;   // [B, H, T, D] order: blocks per (batch, slot)
   int64_t tokens;        // B * T
   float sgn;
 };
@@ -74,79 +77,80 @@ __device__ __forceinline__ int axis_of(const Axes& ax, int pair) {
   return a;
 }
 
-template <typename T, typename C, typename P, int VEC, bool HEAD_MAJOR>
+// Block: g.tokens_block tokens of all heads. Its threads first fetch one
+// (cos, sin) each into LDS, while their first heads' loads are in flight.
+template <typename T, typename C, typename P, int VEC, bool HEAD_MAJOR, int UNROLL>
 __global__ __launch_bounds__(kThreads) void rope_axes_kernel(T* __restrict__ q_out, const T* __restrict__ q_in,
                                                              T* __restrict__ k_out, const T* __restrict__ k_in,
                                                              const C* __restrict__ cosp, const C* __restrict__ sinp,
                                                              RopeAxesArgs g) {
-  const uint32_t lane_c = threadIdx.x % g.lanes;
+  __shared__ __align__(16) float angle[2][kThreads * VEC];  // cos and sin of [token of the block][pair]
+  const uint32_t lane = threadIdx.x % g.lanes;
   const uint32_t rest = threadIdx.x / g.lanes;
-  const uint32_t chunk = blockIdx.y * g.lanes + lane_c;
-  int64_t b;
-  uint32_t t, slot;
-  if constexpr (HEAD_MAJOR) {
-    const uint32_t group = blockIdx.x / g.blocks_row;
-    t = (blockIdx.x % g.blocks_row) * g.tokens_block + rest;
-    slot = group % g.slots;
-    b = group / g.slots;
-    if (rest >= g.tokens_block || t >= g.T || chunk >= g.chunks) return;
-  } else {
-    const uint32_t local = rest / g.slots;
-    slot = rest % g.slots;
-    const int64_t n = (int64_t)blockIdx.x * g.tokens_block + local;
-    if (local >= g.tokens_block || n >= g.tokens || chunk >= g.chunks) return;
-    b = (uint32_t)n / g.T;
-    t = (uint32_t)n % g.T;
-  }
+  const uint32_t local = HEAD_MAJOR ? rest % g.tokens_block : rest / g.slots;
+  const uint32_t slot = HEAD_MAJOR ? rest / g.tokens_block : rest % g.slots;
+  const uint32_t chunk = blockIdx.y * g.lanes + lane;
+  const int64_t n = (int64_t)blockIdx.x * g.tokens_block + local;
+  const bool live = local < g.tokens_block && slot < g.slots && n < g.tokens && chunk < g.chunks;
+  const uint32_t b = live ? (uint32_t)n / g.T : 0, t = live ? (uint32_t)n % g.T : 0;
   const int first = (int)chunk * VEC;
+  const int heads = live ? g.q.count + g.k.count : 0;
 
-  // cos/sin of this lane's pairs, an axis at a time
-  float c[VEC], s[VEC];
-  int axis[VEC];
+  Pack<T, VEC> p1[UNROLL], p2[UNROLL];
+  T* out[UNROLL];
+  const int64_t iq = b * g.q.is_b + t * g.q.is_t + first, ik = b * g.k.is_b + t * g.k.is_t + first;
+  const int64_t oq = b * g.q.os_b + t * g.q.os_t + first, ok = b * g.k.os_b + t * g.k.os_t + first;
+  auto load = [&](int h0) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) axis[i] = axis_of(g.axes, first + i);
-  const P* pos = static_cast<const P*>(g.positions) + b * g.ps_b + t * g.ps_t;
-#pragma unroll
-  for (int a = 0; a < kMaxAxes; ++a) {
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) any = any || axis[i] == a;
-    if (a < g.axes.count && any) {
-      const int64_t at = (int64_t)pos[a * g.ps_a];
-      const bool in = at >= 0 && at < g.table_rows;
-      float ca[VEC], sa[VEC];
-      if (in) {
-        unpack(load_pack<C, VEC>(cosp + at * g.table_ld + first), ca);
-        unpack(load_pack<C, VEC>(sinp + at * g.table_ld + first), sa);
+    for (int j = 0; j < UNROLL; ++j) {
+      const int h = h0 + j * (int)g.slots;
+      if (h < heads) {
+        const T* in = h < g.q.count ? q_in + (iq + h * g.q.is_h) : k_in + (ik + (h - g.q.count) * g.k.is_h);
+        out[j] = h < g.q.count ? q_out + (oq + h * g.q.os_h) : k_out + (ok + (h - g.q.count) * g.k.os_h);
+        p1[j] = load_pack<T, VEC>(in);
+        p2[j] = load_pack<T, VEC>(in + g.half);
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (axis[i] == a) {
-          c[i] = in ? ca[i] : __builtin_nanf("");
-          s[i] = in ? sa[i] * g.sgn : __builtin_nanf("");
-        }
+    }
+  };
+  load((int)slot);
+  const int at = (int)(local * g.lanes + lane) * VEC;
+  if (live) {
+    const P* pos = static_cast<const P*>(g.positions) + b * g.ps_b + t * g.ps_t;
+    for (int i = (int)slot; i < VEC; i += (int)g.slots) {
+      const int64_t p = (int64_t)pos[axis_of(g.axes, first + i) * g.ps_a];
+      float c = __builtin_nanf(""), s = c;
+      if (p >= 0 && p < g.table_rows) {
+        c = to_f32<C>(cosp[p * g.table_ld + first + i]);
+        s = to_f32<C>(sinp[p * g.table_ld + first + i]) * g.sgn;
       }
+      angle[0][at + i] = c;
+      angle[1][at + i] = s;
     }
   }
-
-  const int heads = g.q.count + g.k.count;
-  for (int h = (int)slot; h < heads; h += (int)g.slots) {
-    const bool is_q = h < g.q.count;
-    const int hh = is_q ? h : h - g.q.count;
-    const T* in = (is_q ? q_in : k_in) + b * (is_q ? g.q.is_b : g.k.is_b) + hh * (is_q ? g.q.is_h : g.k.is_h) +
-                  t * (is_q ? g.q.is_t : g.k.is_t) + first;
-    T* out = (is_q ? q_out : k_out) + b * (is_q ? g.q.os_b : g.k.os_b) + hh * (is_q ? g.q.os_h : g.k.os_h) +
-             t * (is_q ? g.q.os_t : g.k.os_t) + first;
-    float x1[VEC], x2[VEC], y1[VEC], y2[VEC];
-    unpack(load_pack<T, VEC>(in), x1);
-    unpack(load_pack<T, VEC>(in + g.half), x2);
+  __syncthreads();
+  if (!live) return;
+  float c[VEC], s[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      y1[i] = x1[i] * c[i] - x2[i] * s[i];
-      y2[i] = x2[i] * c[i] + x1[i] * s[i];
+  for (int i = 0; i < VEC; ++i) c[i] = angle[0][at + i], s[i] = angle[1][at + i];
+
+  for (int h0 = (int)slot; h0 < heads;) {
+#pragma unroll
+    for (int j = 0; j < UNROLL; ++j) {
+      if (h0 + j * (int)g.slots < heads) {
+        float x1[VEC], x2[VEC], y1[VEC], y2[VEC];
+        unpack(p1[j], x1);
+        unpack(p2[j], x2);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          y1[i] = x1[i] * c[i] - x2[i] * s[i];
+          y2[i] = x2[i] * c[i] + x1[i] * s[i];
+        }
+        store_pack_nt<T, VEC>(out[j], pack<T, VEC>(y1));
+        store_pack_nt<T, VEC>(out[j] + g.half, pack<T, VEC>(y2));
+      }
     }
-    store_pack<T, VEC>(out, pack<T, VEC>(y1));
-    store_pack<T, VEC>(out + g.half, pack<T, VEC>(y2));
+    h0 += (int)g.slots * UNROLL;
+    load(h0);
   }
 }
 
@@ -247,23 +251,20 @@ int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int
         g.lanes = std::min<uint32_t>(g.chunks, kThreads);
         const uint32_t per_block = kThreads / g.lanes;
         const int64_t heads = Hq + Hk;
-        g.slots = (uint32_t)std::min<int64_t>(heads, head_major ? heads : per_block);
-        dim3 grid(1, (unsigned)cdiv((int64_t)g.chunks, (int64_t)g.lanes));
-        int64_t blocks;
-        if (head_major) {
-          g.tokens_block = per_block;
-          g.blocks_row = (uint32_t)cdiv(T, (int64_t)per_block);
-          blocks = B * (int64_t)g.slots * g.blocks_row;
-        } else {
-          g.tokens_block = per_block / g.slots;
-          blocks = cdiv(g.tokens, (int64_t)g.tokens_block);
-        }
-        HK_REQUIRE(blocks < (1LL << 31), "too many rows for one launch");
-        grid.x = (unsigned)blocks;
+        // Tokens a block. Eight slots (a lane walks heads / 8 heads with one set of angles) once that leaves about
+        // four blocks a CU; fewer tokens and more slots before that, so that a few tokens still spread over the GPU
+        // (64 tokens x 40 heads: one block a token). 8 slots of 8 lanes: 31.4 us for q and k of 8192 tokens x 40
+        // heads x 128 bf16 (4 slots 34, 20 slots 33 and more; a copy of the same bytes 30.2).
+        uint32_t tb = (uint32_t)std::max<int64_t>(1, per_block / heads);
+        while (tb * 16 <= per_block && g.tokens >= (int64_t)tb * 2048) tb *= 2;
+        g.tokens_block = tb;
+        g.slots = (uint32_t)std::min<int64_t>(heads, per_block / tb);
+        const int64_t blocks = cdiv(g.tokens, (int64_t)tb);
+        const dim3 grid((unsigned)blocks, (unsigned)cdiv((int64_t)g.chunks, (int64_t)g.lanes));
         auto go = [&](auto tp, auto order) {
           using TP = typename decltype(tp)::type;
           constexpr bool HM = decltype(order)::value;
-          hipLaunchKernelGGL((rope_axes_kernel<TX, TC, TP, VEC, HM>), grid, dim3(kThreads), 0, st, (TX*)q_out,
+          hipLaunchKernelGGL((rope_axes_kernel<TX, TC, TP, VEC, HM, 2>), grid, dim3(kThreads), 0, st, (TX*)q_out,
                              (const TX*)q_in, (TX*)k_out, (const TX*)k_in, (const TC*)cos, (const TC*)sin, g);
           return check_launch("rope_axes_kernel");
         };
@@ -273,9 +274,11 @@ int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int
       };
       constexpr int V = 16 / sizeof(TX);
       const bool whole = half % V == 0 && heads_ok(g.q, q_in, q_out, V, sizeof(TX)) &&
-                         heads_ok(g.k, k_in, k_out, V, sizeof(TX)) && table_ld % V == 0 &&
-                         aligned_to(cos, sizeof(TC) * V) && aligned_to(sin, sizeof(TC) * V);
+                         heads_ok(g.k, k_in, k_out, V, sizeof(TX));
       if (whole) return launch(std::integral_constant<int, V>{});
+      const bool halves = half % (V / 2) == 0 && heads_ok(g.q, q_in, q_out, V / 2, sizeof(TX)) &&
+                          heads_ok(g.k, k_in, k_out, V / 2, sizeof(TX));
+      if (halves) return launch(std::integral_constant<int, V / 2>{});  // (D = 72 in 16 bits)
       return launch(std::integral_constant<int, 1>{});
     });
   });

@@ -128,9 +128,12 @@ def call(name: str, *args) -> None:
 
 
 def call_on(device: torch.device, name: str, *args) -> None:
-    """``call`` with the device's current stream as the last argument, that device being made current for the launch."""
-    if device.index is None or device.index == torch._C._cuda_getDevice():
-        call(name, *args, stream_of(device))
+    """``call`` with the device's current stream as the last argument, that device being current during the call."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = getattr(_lib or load(), name)(*args, torch._C._cuda_getCurrentRawStream(index))
+        if status:
+            check(status, name)
         return
     with torch.cuda.device(device):
         call(name, *args, stream_of(device))

@@ -34,53 +34,49 @@ def _sections_arg(sections):
     return arr
 
 
-def _table(t):
-    """(rows, D/2) of a cos or sin table given as that or as (1, rows, D/2)."""
-    if t.dim() == 3:
-        assert t.shape[0] == 1, f"cos/sin must be (1, positions, head_dim/2); got {tuple(t.shape)}"
-        t = t[0]
-    assert t.dim() == 2, f"cos/sin must be (1, positions, head_dim/2); got {tuple(t.shape)}"
-    return t if t.stride(1) == 1 else t.contiguous()
-
-
-def _rows(x):
-    """x with unit stride in the head dim."""
-    return x if x.stride(-1) == 1 else x.contiguous()
-
-
 def _launch(q, k, cos, sin, positions, sections, interleaved, inverse):
     """(q_out, k_out): one launch over both."""
+    # shapes and strides are read once each (host time: a decode step's call is bound by it)
     dev = _lib.require_device(q, k, cos, sin, positions)
-    assert q.dim() == 4 and k.dim() == 4, "q and k must be (bsz, n_heads, seq_len, head_dim)"
-    bsz, hq, seq_len, hd = q.shape
-    kb, hk, kt, kd = k.shape
-    assert (kb, kt, kd) == (bsz, seq_len, hd), f"q and k differ: {tuple(q.shape)} and {tuple(k.shape)}"
-    assert q.dtype == k.dtype, f"q and k have different dtypes: {q.dtype} and {k.dtype}"
-    cos, sin = _table(cos), _table(sin)
-    assert cos.shape == sin.shape and cos.dtype == sin.dtype, "cos and sin must be alike"
-    assert cos.shape[1] * 2 == hd, f"cos/sin must be (1, positions, head_dim/2); got {tuple(cos.shape)}"
-    if cos.stride() != sin.stride():
-        cos, sin = cos.contiguous(), sin.contiguous()
+    qs, ks, cs, ps = q.shape, k.shape, cos.shape, positions.shape
+    assert len(qs) == 4 and len(ks) == 4, "q and k must be (bsz, n_heads, seq_len, head_dim)"
+    bsz, hq, seq_len, hd = qs
+    kb, hk, kt, kd = ks
+    assert kb == bsz and kt == seq_len and kd == hd, f"q and k differ: {tuple(qs)} and {tuple(ks)}"
+    dtype, table_dtype = q.dtype, cos.dtype
+    assert k.dtype == dtype, f"q and k have different dtypes: {dtype} and {k.dtype}"
+    assert sin.shape == cs and sin.dtype == table_dtype, "cos and sin must be alike"
+    assert (len(cs) == 2 or len(cs) == 3 and cs[0] == 1) and cs[-1] * 2 == hd, \
+        f"cos/sin must be (1, positions, head_dim/2); got {tuple(cs)}"
     sec = _sections_arg(sections)
     axes = len(sec)
-    if positions.dtype not in _POS_CODE:
+    pos_code = _POS_CODE.get(positions.dtype)
+    if pos_code is None:
         raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    assert positions.dim() == 3 and positions.shape[0] == axes and positions.shape[2] == seq_len and \
-        positions.shape[1] in (1, bsz), \
-        f"positions must be ({axes}, {bsz} or 1, {seq_len}); got {tuple(positions.shape)}"
+    assert len(ps) == 3 and ps[0] == axes and ps[2] == seq_len and (ps[1] == bsz or ps[1] == 1), \
+        f"positions must be ({axes}, {bsz} or 1, {seq_len}); got {tuple(ps)}"
     pa, pb, pt = positions.stride()
-    if positions.shape[1] == 1:
+    if ps[1] == 1:
         pb = 0
-    q, k = _rows(q), _rows(k)
+    cst = cos.stride()
+    if cst[-1] != 1 or sin.stride() != cst:
+        cos, sin = cos.contiguous(), sin.contiguous()
+        cst = cos.stride()
+    qi, ki = q.stride(), k.stride()
+    if qi[3] != 1:
+        q = q.contiguous()
+        qi = q.stride()
+    if ki[3] != 1:
+        k = k.contiguous()
+        ki = k.stride()
     # empty_like keeps a dense input's layout and is contiguous for broadcast (zero-stride) ones
     q_out, k_out = torch.empty_like(q), torch.empty_like(k)
-    qi, ki, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
+    qo, ko = q_out.stride(), k_out.stride()
     assert qo[3] == 1 and ko[3] == 1
     _lib.call_on(dev, "hk_rope_axes", q_out.data_ptr(), q.data_ptr(), hq, qi[0], qi[1], qi[2], qo[0], qo[1], qo[2],
                  k_out.data_ptr(), k.data_ptr(), hk, ki[0], ki[1], ki[2], ko[0], ko[1], ko[2],
-                 cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.stride(0), positions.data_ptr(),
-                 _POS_CODE[positions.dtype], pa, pb, pt, sec, axes, int(interleaved), bsz, seq_len, hd,
-                 _lib.dtype_code(q), _lib.dtype_code(cos), int(inverse))
+                 cos.data_ptr(), sin.data_ptr(), cs[-2], cst[-2], positions.data_ptr(), pos_code, pa, pb, pt, sec, axes,
+                 interleaved, bsz, seq_len, hd, _lib.dtype_code(q), _lib.dtype_code(cos), inverse)
     return q_out, k_out
 
 
