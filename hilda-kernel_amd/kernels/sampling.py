@@ -14,19 +14,21 @@ from . import _lib
 _TOP_K_CODE = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 
 
-def _rows_of(t, shape, name):
+def _rows_of(t, shape, name, device=None):
     """A per-row setting as a contiguous tensor of the rows."""
     assert t.shape == shape, f"{name} must have one value for each row {tuple(shape)}, got {tuple(t.shape)}"
+    if device is not None and t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, the logits on {device}")
     return t.contiguous()
 
 
-def _setting(value, shape, name):
+def _setting(value, shape, name, device):
     """(tensor or None, number) of a float setting."""
     if not isinstance(value, torch.Tensor):
         return None, float(value)
     if value.dtype != torch.float32:
         raise TypeError(f"{name} must be float32, got {value.dtype}")
-    return _rows_of(value, shape, name), 0.0
+    return _rows_of(value, shape, name, device), 0.0
 
 
 @torch.no_grad()
@@ -51,23 +53,26 @@ def hilda_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     if uniform.dtype != torch.float32:
         raise TypeError(f"uniform must be float32, got {uniform.dtype}")
     uniform = _rows_of(uniform, shape, "uniform")
-    t_rows, t = _setting(temperature, shape, "temperature")
-    p_rows, p = _setting(top_p, shape, "top_p")
-    m_rows, m = _setting(min_p, shape, "min_p")
+    t_rows, t = _setting(temperature, shape, "temperature", dev)
+    p_rows, p = _setting(top_p, shape, "top_p", dev)
+    m_rows, m = _setting(min_p, shape, "min_p", dev)
     k_rows, k, k_code = None, 0, 0
     if isinstance(top_k, torch.Tensor):
         if top_k.dtype not in _TOP_K_CODE:
             raise TypeError(f"top_k must be int32 or int64, got {top_k.dtype}")
-        k_rows, k_code = _rows_of(top_k, shape, "top_k"), _TOP_K_CODE[top_k.dtype]
+        k_rows, k_code = _rows_of(top_k, shape, "top_k", dev), _TOP_K_CODE[top_k.dtype]
     else:
         k = min(max(int(top_k), 0), vocab)
-    _lib.require_device(logits, t_rows, k_rows, p_rows, m_rows)
-    if logits.dim() != 2 or logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < vocab):
+    strides = logits.stride()
+    if len(strides) != 2 or strides[1] != 1 or strides[0] < vocab:
         logits = logits.reshape(-1, vocab).contiguous()
     rows = logits.shape[0]
     ids = torch.empty(shape, dtype=torch.int64, device=dev)
     logp = torch.empty(shape, dtype=torch.float32, device=dev)
+    cuts = k_rows is not None or p_rows is not None or 0 < k < vocab or p < 1
+    nbytes = _lib.load().hk_sample_workspace_size(rows, vocab, cuts, dev.index)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "hk_sample", ids.data_ptr(), logp.data_ptr(), logits.data_ptr(), uniform.data_ptr(), rows, vocab,
                  logits.stride(0) if rows > 1 else vocab, _lib.ptr(t_rows), t, _lib.ptr(k_rows), k_code, k,
-                 _lib.ptr(p_rows), p, _lib.ptr(m_rows), m, _lib.dtype_code(logits))
+                 _lib.ptr(p_rows), p, _lib.ptr(m_rows), m, _lib.dtype_code(logits), ws.data_ptr(), nbytes)
     return ids, logp

@@ -390,7 +390,11 @@ int hk_selective_log_softmax(float* logp, const void* logits, const int64_t* ids
 int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int64_t rows, int64_t cols, int64_t ld,
               const float* temperature_rows, double temperature, const void* top_k_rows, int top_k_type, int64_t top_k,
               const float* top_p_rows, double top_p, const float* min_p_rows, double min_p, int dtype,
-              hk_stream_t stream);
+              void* workspace, size_t workspace_bytes, hk_stream_t stream);
+
+/* Bytes of hk_sample's workspace (16-byte aligned) on `device`; cuts: whether
+ * top-k or top-p may be on (a pointer given, 0 < top_k < cols or top_p < 1). */
+size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int device);
 
 /* Bytes of device workspace hk_grpo_loss_fwd needs. */
 size_t hk_grpo_workspace_size(int64_t B, int64_t L);

@@ -18,7 +18,7 @@ import torch
 import oracle
 from _util import gpu
 
-from kernels import fused_selective_log_softmax, hilda_grpo_loss, hilda_sample
+from kernels import _lib, fused_selective_log_softmax, hilda_grpo_loss, hilda_sample
 
 pytestmark = pytest.mark.gpu
 
@@ -264,3 +264,18 @@ def test_refusals(bad):
         u = u.cpu()
     with pytest.raises((AssertionError, TypeError, ValueError, RuntimeError)):
         hilda_sample(x, u, **kw)
+
+
+def test_workspace_is_checked():
+    dev = gpu()
+    x, u = torch.zeros(4, 5000, device=dev), torch.zeros(4, device=dev)
+    ids, logp = torch.empty(4, dtype=torch.int64, device=dev), torch.empty(4, device=dev)
+    need = _lib.load().hk_sample_workspace_size(4, 5000, 1, dev.index)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    for nbytes, ok in ((need, True), (need - 256, False)):
+        status = _lib.load().hk_sample(ids.data_ptr(), logp.data_ptr(), x.data_ptr(), u.data_ptr(), 4, 5000, 5000, None, 1.0,
+                                       None, 0, 7, None, 1.0, None, 0.0, _lib.F32, ws.data_ptr(), nbytes,
+                                       _lib.stream_of(dev))
+        assert (status == 0) == ok
+    assert "workspace too small" in _lib.last_error()
+    assert ids.tolist() == [0] * 4

@@ -178,9 +178,9 @@ def test_sample_refusals():
     lib = _lib.load()
     p = ctypes.c_void_p(256)
 
-    def call(ids=p, rows=4, cols=100, ld=100, t=1.0, k_rows=None, k_type=0, top_p=1.0, min_p=0.0, dtype=2):
+    def call(ids=p, rows=4, cols=100, ld=100, t=1.0, k_rows=None, k_type=0, top_p=1.0, min_p=0.0, dtype=2, ws=p):
         return lib.hk_sample(ids, p, p, p, rows, cols, ld, None, t, k_rows, k_type, 0, None, top_p, None, min_p, dtype,
-                             None)
+                             ws, 1 << 20, None)
 
     _einval(call(dtype=5), "dtype")
     _einval(call(rows=-1), "shape")
@@ -194,4 +194,11 @@ def test_sample_refusals():
         _einval(call(min_p=v), "min_p")
     _einval(call(k_rows=p, k_type=_lib.F32), "top_k")
     _einval(call(ids=None), "null")
+    _einval(call(ws=None), "workspace")
+    _einval(call(ws=ctypes.c_void_p(264)), "aligned")
     assert call(rows=0) == 0
+    # more for the cuts' bins, nothing that grows with rows * cols but the runs' records
+    small, large = (lib.hk_sample_workspace_size(256, 151936, cuts, 0) for cuts in (0, 1))
+    assert 0 < small < large < 64 * 2 ** 20
+    assert lib.hk_sample_workspace_size(1 << 20, 300, 1, 0) < 64 * 2 ** 20
+    assert lib.hk_sample_workspace_size(-1, 300, 1, 0) == lib.hk_sample_workspace_size(4, 0, 1, 0) == 0
