@@ -48,15 +48,14 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int kRun = 2048;            // columns of a run: 32 a lane
-constexpr int kLaneCols = kRun / kWave;
-constexpr int kLanes = 512;           // threads of a block (pick: kPickLanes)
+constexpr int kLanes = 1024;          // threads of a block
 constexpr int kWaves = kLanes / kWave;
-constexpr int kPickLanes = 256;
 constexpr int kMaxSplit = 16;         // blocks a row
-constexpr int kBins = 2048;
+constexpr int kFineBins = 2048;
 // the linear bins cover max - x < kRange * T; beyond it is one bin
 constexpr double kRange = 24;
 constexpr double kTempMin = 0x1p-64, kTempMax = 0x1p64;
+constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 constexpr int kMaxQuarters = 1024;    // quarter maxima that a bound on the k-th logit is taken from
 
 // A setting of every row, or one each.
@@ -64,9 +63,44 @@ struct Setting {
   const float* rows;
   double all;
 };
-struct Hist {
-  u64 mass[kBins];
-  uint32_t count[kBins];
+
+// Bins of logits, in descending order. fp32 and fp16: linear in max - x, with counts and masses. bf16: one bin for each
+// value of 2^-12 <= |x| < 2^8 (kSide of either sign), so a count is a mass, and three more that hold several: x >= 2^8,
+// |x| < 2^-12 and x <= -2^8.
+template <typename T> struct Bins {
+  static constexpr int kCount = 2048, kMasses = kCount;
+  static constexpr bool kExact = false;
+};
+template <> struct Bins<__bf16> {
+  static constexpr int kSide = 20 * 128, kLowest = (127 - 12) << 7;  // kLowest: the bits of 2^-12
+  static constexpr int kZero = kSide + 1, kUsed = 2 * kSide + 3;
+  static constexpr int kCount = 6144, kMasses = 4;  // (whole turns of the block; masses of the three)
+  static constexpr bool kExact = true;
+  static __device__ __forceinline__ int of(float v) {
+    const int b = (int)f32_bits(v), sign = b >> 31;
+    const int i = ::min(::max(((b >> 16) & 0x7fff) - kLowest + 1, 0), kSide + 1);
+    return kZero - (i ^ sign) + sign;
+  }
+  // of both bf16 values of a word, by packed 16-bit integers; `rank`: 0 for |x| < 2^-12, kSide + 1 for |x| >= 2^8
+  typedef short Two __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ Two of_two(uint32_t w, Two* rank) {
+    const Two sign = __builtin_bit_cast(Two, w) >> (short)15;
+    const Two i = __builtin_elementwise_min(
+        __builtin_elementwise_max((Two)(__builtin_bit_cast(Two, w & 0x7fff7fffu) - (short)(kLowest - 1)), (Two)((short)0)),
+        (Two)((short)(kSide + 1)));
+    *rank = i;
+    return (short)kZero - (i ^ sign) + sign;
+  }
+  static __device__ __forceinline__ bool several(int bin) { return bin == 0 || bin == kZero || bin == kUsed - 1; }
+  static __device__ __forceinline__ int slot(int bin) { return bin == 0 ? 0 : bin == kZero ? 1 : 2; }
+  static __device__ __forceinline__ float value(int bin) {
+    const int i = bin < kZero ? kZero - bin : bin - kZero;
+    return bits_f32((uint32_t)(kLowest + i - 1) << 16 | (bin < kZero ? 0u : 0x80000000u));
+  }
+};
+template <typename T> struct Hist {
+  u64 mass[Bins<T>::kMasses];
+  uint32_t count[Bins<T>::kCount];
 };
 // A cut: logits above x are kept, and the first `ties` of those equal to x
 // (of `equal` in the row; all of them if ties >= equal).
@@ -86,14 +120,15 @@ struct SampleArgs {
   int64_t ld;
   int cols, runs;  // runs of a row
   int split;       // blocks of a row
+  int has_cuts;    // cuts is written
   double magic;    // 2^(52 - b): e + magic holds e in b fixed-point bits
   // workspace
   float *part_max, *part_sum;  // [rows][split]
   float* quarters;             // [rows][4 runs] maxima of 512 columns
   double* run_mass;            // [rows][runs]
   uint32_t* run_ties;
-  float* run_max;
-  Hist* hist;                  // [rows][split], split > 1
+  float *run_max, *run_ref;    // of open rows: the run's maximum, and the logit whose mass its masses take as 1
+  void* hist;                  // Hist<T> [rows][split], split > 1
   Cut* cuts;                   // [rows]
 };
 
@@ -102,12 +137,14 @@ __device__ __forceinline__ double setting(const Setting& s, int64_t row) { retur
 // What a row asks for.
 struct Asked {
   double temp, top_p, min_p;
+  double k;  // log2(e) / T
   int64_t top_k;
   bool by_k, by_p, open;  // open: no filter at all
   bool in_range;
 };
 __device__ __forceinline__ Asked asked(const SampleArgs& g, int64_t row) {
   Asked a;
+  const float u = g.u[row];
   a.temp = setting(g.temperature, row);
   a.top_p = setting(g.top_p, row);
   a.min_p = setting(g.min_p, row);
@@ -115,17 +152,17 @@ __device__ __forceinline__ Asked asked(const SampleArgs& g, int64_t row) {
   if (g.top_k_rows)
     a.top_k = g.top_k_wide ? static_cast<const int64_t*>(g.top_k_rows)[row]
                            : static_cast<const int32_t*>(g.top_k_rows)[row];
+  a.k = kLog2eD / a.temp;
   a.by_k = a.top_k > 0 && a.top_k < g.cols;
   a.by_p = a.top_p < 1.0;
   a.open = !a.by_k && !a.by_p && !(a.min_p > 0.0);
-  const float u = g.u[row];
   a.in_range = a.temp >= kTempMin && a.temp <= kTempMax && u >= 0.f && u <= 1.f && a.top_p == a.top_p &&
                a.min_p == a.min_p;
   return a;
 }
 
-// 2^y for y <= 0: y = n + r, |r| <= 1/2 (n from the low bits of y + 1.5 * 2^52), and for 2^r the polynomial of degree
-// 10 that interpolates it at the Chebyshev nodes of [-1/2, 1/2] (relative error 3.2e-16). y = d * k with one rounding.
+// 2^y: y = n + r, |r| <= 1/2 (n from the low bits of y + 1.5 * 2^52), and for 2^r the polynomial of degree 10 that
+// interpolates it at the Chebyshev nodes of [-1/2, 1/2] (relative error 3.2e-16). y = d * k with one rounding.
 // 0 below y = -1080; NaN stays NaN.
 __device__ __forceinline__ double exp2_product(double d, double k) {
   constexpr double kShift = 6755399441055744.0;
@@ -166,65 +203,83 @@ template <typename T> __device__ __forceinline__ float value_of(uint32_t key) {
   return bits_f32(~(k | (uint32_t)((1ull << S) - 1)));
 }
 
-// This lane's 32 logits of a run; column of v[i]: run * kRun + col_of(i). -inf past the row's end (no filter and no sum
-// tells those from masked tokens).
+// VEC logits from column c; -inf past the row's end (no filter and no sum tells those from masked tokens)
 template <typename T>
-struct Run {
-  static constexpr int VEC = 16 / sizeof(T);
-  float v[kLaneCols];
-  __device__ __forceinline__ void load(const T* row, int run, int cols) {
-    const int lane = threadIdx.x % kWave;
-    const int c0 = run * kRun + lane * VEC;
-    if ((run + 1) * kRun <= cols) {  // (the same for the whole wave)
-      Pack<T, VEC> p[kLaneCols / VEC];
+__device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_cols(const T* row, int c, int cols) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (c + VEC <= cols) return load_pack_any<T, VEC>(row + c);
+  float f[VEC];
 #pragma unroll
-      for (int j = 0; j < kLaneCols / VEC; ++j) p[j] = load_pack_any<T, VEC>(row + c0 + j * kWave * VEC);
-#pragma unroll
-      for (int j = 0; j < kLaneCols / VEC; ++j) {
-        float f[VEC];
-        unpack(p[j], f);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j * VEC + i] = f[i];
-      }
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < kLaneCols / VEC; ++j) {
-      const int c = c0 + j * kWave * VEC;
-      float f[VEC];
-      if (c + VEC <= cols) {
-        unpack(load_pack_any<T, VEC>(row + c), f);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) f[i] = c + i < cols ? to_f32<T>(row[c + i]) : -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j * VEC + i] = f[i];
-    }
-  }
-  __device__ __forceinline__ float lane_max() const {
-    float m = v[0];
-#pragma unroll
-    for (int i = 1; i < kLaneCols; ++i) m = fmaxf(m, v[i]);
-    return m;
-  }
-};
+  for (int i = 0; i < VEC; ++i) f[i] = c + i < cols ? to_f32<T>(row[c + i]) : -INFINITY;
+  return pack<T, VEC>(f);
+}
 
-template <typename X> __device__ __forceinline__ X wave_total(X v) {
-#pragma unroll
-  for (int o = 1; o < kWave; o *= 2) v += __shfl_xor(v, o, kWave);
-  return v;
-}
-template <typename X> __device__ __forceinline__ X wave_scan(X v) {  // inclusive
-  const int lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int o = 1; o < kWave; o *= 2) {
-    const X t = __shfl_up(v, o, kWave);
-    if (lane >= o) v += t;
+// A row's runs first, first + waves, ...: look(pack, column) for each 16 bytes of a lane, done(run) after each run. A
+// wave has two packs on their way. The loop stays rolled: unrolled over a run (32 logits a lane) these kernels have 25
+// to 80 KB of code, and fetching it, not the logits, set their time (hist of 64 x 151936: 33 us; 11 rolled).
+template <typename T, typename L, typename D>
+__device__ __forceinline__ void each_run(const T* row, int cols, int runs, int first, int waves, L&& look, D&& done) {
+  constexpr int VEC = 16 / sizeof(T), kStep = kWave * VEC, kPacks = kRun / kStep;
+  if (first >= runs) return;
+  const int lane_col = (int)(threadIdx.x % kWave) * VEC;
+  int ahead = first, ahead_pack = 2;
+  Pack<T, VEC> p0 = load_cols(row, first * kRun + lane_col, cols);
+  Pack<T, VEC> p1 = load_cols(row, first * kRun + kStep + lane_col, cols);
+  for (int run = first; run < runs; run += waves) {
+#pragma unroll 1
+    for (int j = 0; j < kPacks; ++j) {
+      const Pack<T, VEC> p = p0;
+      p0 = p1;
+      if (ahead_pack == kPacks) ahead_pack = 0, ahead += waves;
+      if (ahead < runs) p1 = load_cols(row, ahead * kRun + ahead_pack * kStep + lane_col, cols);
+      ++ahead_pack;
+      look(p, run * kRun + j * kStep + lane_col);
+    }
+    done(run);
   }
+}
+
+// A value moved between lanes by the DPP pattern CTRL, word by word; lanes without a source, and rows outside ROW_MASK,
+// get 0.
+template <int CTRL, int ROW_MASK = 0xf, typename X>
+__device__ __forceinline__ X moved(X v) {
+  if constexpr (sizeof(X) == 4) {
+    return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROW_MASK, 0xf, false));
+  } else {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(X, u32x2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, ROW_MASK, 0xf, false),
+                                       (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, ROW_MASK, 0xf, false)});
+  }
+}
+template <typename X> __device__ __forceinline__ X of_lane63(X v) {
+  if constexpr (sizeof(X) == 4) {
+    return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+  } else {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(X, u32x2{(uint32_t)__builtin_amdgcn_readlane((int)w.x, 63),
+                                       (uint32_t)__builtin_amdgcn_readlane((int)w.y, 63)});
+  }
+}
+// inclusive, over the wave: within rows of 16 lanes (row_shr 1, 2, 4, 8), then across them
+template <typename X> __device__ __forceinline__ X wave_scan(X v) {
+  v += moved<0x111>(v);
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  v += moved<0x118>(v);
+  v += moved<dpp::kBcast15, 0xa>(v);
+  v += moved<dpp::kBcast31, 0xc>(v);
   return v;
 }
-// sum over the threads before this one; `tmp` holds one value a wave
+template <typename X> __device__ __forceinline__ X wave_total(X v) {
+  v += moved<dpp::kXor1>(v);
+  v += moved<dpp::kXor2>(v);
+  v += moved<dpp::kHalfMirror>(v);
+  v += moved<dpp::kMirror>(v);
+  v += moved<dpp::kBcast15, 0xa>(v);
+  v += moved<dpp::kBcast31, 0xc>(v);
+  return of_lane63(v);
+}
+// sum over the threads before this one; `tmp` holds one value a wave and, after it, their totals
 template <typename X> __device__ __forceinline__ X block_before(X v, X* tmp) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const X incl = wave_scan(v);
@@ -232,87 +287,234 @@ template <typename X> __device__ __forceinline__ X block_before(X v, X* tmp) {
   if (lane == kWave - 1) tmp[wave] = incl;
   __syncthreads();
   X before = incl - v;
+#pragma unroll 1
   for (int i = 0; i < wave; ++i) before += tmp[i];
   return before;
 }
+template <typename X> __device__ __forceinline__ X total_of(const X* tmp) {
+  X t = tmp[0];
+#pragma unroll 1
+  for (int i = 1; i < kWaves; ++i) t += tmp[i];
+  return t;
+}
 
-// A row's maximum and sum of e^(z - max) from its blocks' parts (split <= 64); false if it has no distribution. Every
-// wave computes it for itself.
-__device__ __forceinline__ bool row_state(const SampleArgs& g, int64_t row, const Asked& a, float* max, float* sum) {
-  const int lane = threadIdx.x % kWave;
-  const float m = lane < g.split ? g.part_max[row * g.split + lane] : -INFINITY;
-  const float s = lane < g.split ? g.part_sum[row * g.split + lane] : 0.f;
-  const float c = (float)(1.4426950408889634074 / a.temp);
-  *max = wave_max(m);
-  *sum = wave_sum(m == -INFINITY ? s : s * exp2_fast((m - *max) * c));
-  // (a NaN, a +inf or nothing above -inf leaves the sum NaN or 0)
-  return a.in_range && *sum > 0.f && *sum < INFINITY && *max < INFINITY;
+// The first thread of the block for which `passes`, or if there is none the last for which `some`; -1 without either.
+// `tmp` holds two values a wave.
+__device__ __forceinline__ int first_or_last(bool passes, bool some, int* tmp) {
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const u64 p = __ballot(passes), q = __ballot(some);
+  __syncthreads();
+  if (lane == 0) {
+    tmp[wave] = p ? wave * kWave + __builtin_ctzll(p) : kLanes;
+    tmp[kWaves + wave] = q ? wave * kWave + 63 - __builtin_clzll(q) : -1;
+  }
+  __syncthreads();
+  int first = kLanes, last = -1;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) first = min(first, tmp[i]), last = max(last, tmp[kWaves + i]);
+  return first < kLanes ? first : last;
+}
+
+// What the launches after the scan begin with, its loads in flight together: the row's settings, its maximum and sum of
+// e^(z - max) from its blocks' parts (every wave puts them together for itself), and its cut. ok: it has a distribution.
+struct Start {
+  Asked a;
+  float max, sum;
+  bool ok;
+  Cut cut;
+  __device__ __forceinline__ Start(const SampleArgs& g, int64_t row, bool with_cut) {
+    const int lane = threadIdx.x % kWave;
+    const float m = lane < g.split ? g.part_max[row * g.split + lane] : -INFINITY;
+    const float s = lane < g.split ? g.part_sum[row * g.split + lane] : 0.f;
+    cut = {-INFINITY, 0xffffffffu, 0};
+    if (with_cut && g.has_cuts) cut = g.cuts[row];
+    a = asked(g, row);
+    if (!a.by_k && !a.by_p) cut = {-INFINITY, 0xffffffffu, 0};
+    max = wave_max(m);
+    sum = wave_sum(m == -INFINITY ? s : s * exp2_fast((m - max) * (float)a.k));
+    // (a NaN, a +inf or nothing above -inf leaves the sum NaN or 0)
+    ok = a.in_range && sum > 0.f && sum < INFINITY && max < INFINITY;
+    if (with_cut && ok && a.min_p > 0.0) {
+      // e^((x - max) / T) >= min_p, as the smallest float that satisfies it. log2 min_p: the instruction's, off by some
+      // 2^-22, and what is left of min_p after it (2^-100 of the largest probability is as good as none).
+      const double p = fmax(fmin(a.min_p, 1.0), 0x1p-100);
+      const double y = (double)log2_fast((float)p), rest = p * exp2_product(-y, 1.0) - 1.0;
+      const double least = (double)max + a.temp * kLn2D * (y + kLog2eD * (rest - 0.5 * rest * rest));
+      float f = (float)(p < 1.0 ? least : (double)max);
+      if (p < 1.0 && (double)f < least) f = nextafterf(f, INFINITY);
+      if (f > cut.x) cut = {f, 0xffffffffu, 0};
+    }
+  }
+};
+
+// bf16: the masses of the bins that hold one value, 0 in the others, whose logits are looked at one by one.
+template <typename F>
+__device__ __forceinline__ void fill_table(double* table, F&& mass) {
+  typedef Bins<__bf16> B;
+#pragma unroll 1
+  for (int b = threadIdx.x; b < B::kUsed; b += kLanes) table[b] = B::several(b) ? 0.0 : mass(B::value(b));
+  __syncthreads();
+}
+// The sum of the table's masses over a pack, and of `mass` over its logits of the other bins (from column c of the row;
+// those are few). *least: the lowest bin met so far, *most the highest rank.
+template <typename F>
+__device__ __forceinline__ double sum_table(const double* table, const Pack<__bf16, 8>& p, const __bf16* row, int c, int cols,
+                                            int reach, F&& mass) {
+  typedef Bins<__bf16> B;
+  B::Two bins[4], least = (B::Two)((short)B::kUsed), low = (B::Two)((short)B::kSide), high = (B::Two)((short)0);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    B::Two rank;
+    bins[j] = B::of_two(p.w[j], &rank);
+    least = __builtin_elementwise_min(least, bins[j]);
+    low = __builtin_elementwise_min(low, rank);
+    high = __builtin_elementwise_max(high, rank);
+  }
+  double s0 = 0.0, s1 = 0.0;
+  if (__any(min(least.x, least.y) <= reach)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s0 += table[bins[j].x], s1 += table[bins[j].y];
+    if (min(low.x, low.y) == 0 || max(high.x, high.y) > B::kSide) {
+#pragma unroll 1
+      for (int i = c; i < min(c + 8, cols); ++i) {
+        const float v = to_f32<__bf16>(row[i]);
+        if (B::several(B::of(v)) && v != -INFINITY) s0 += mass(v);
+      }
+    }
+  }
+  return s0 + s1;
 }
 
 // ---- scan -------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
+  constexpr int VEC = 16 / sizeof(T);
+  // an open row's masses of bf16 logits below 2^8 in size: 2^(x k) itself from the table, within 2^+-739
+  constexpr bool kTable = Bins<T>::kExact;
+  __shared__ double table[kTable ? Bins<__bf16>::kUsed : 1];
   __shared__ float sm[kWaves], sz[kWaves];
   const int64_t row = blockIdx.x / g.split;
   const int part = blockIdx.x % g.split;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const Asked a = asked(g, row);
   const T* x = static_cast<const T*>(g.logits) + row * g.ld;
-  const double k = 1.4426950408889634074 / a.temp;
-  const float c = (float)k;
-  float m = -INFINITY, z = 0.f;
-  for (int run = part * kWaves + wave; run < g.runs; run += g.split * kWaves) {
-    Run<T> r;
-    r.load(x, run, g.cols);
-    float q = r.lane_max();
-    q = fmaxf(q, dpp_move<dpp::kXor1>(q, q));
-    q = fmaxf(q, dpp_move<dpp::kXor2>(q, q));
-    q = fmaxf(q, dpp_move<dpp::kHalfMirror>(q, q));
-    q = fmaxf(q, dpp_move<dpp::kMirror>(q, q));
-    if (a.by_k && lane % 16 == 0) g.quarters[(row * g.runs + run) * 4 + lane / 16] = q;
-    q = fmaxf(q, dpp_move<dpp::kBcast15, 0xa>(q, q));
-    q = fmaxf(q, dpp_move<dpp::kBcast31, 0xc>(q, q));
-    const float rm = lane63(q);
-    if (a.open) {
-      const double ref = rm == -INFINITY ? 0.0 : (double)rm;
-      double mass = 0.0;
-#pragma unroll
-      for (int i = 0; i < kLaneCols; ++i) mass += exp2_product((double)r.v[i] - ref, k);
-      mass = wave_total(mass);
-      if (lane == 0) g.run_mass[row * g.runs + run] = mass, g.run_max[row * g.runs + run] = rm;
-    } else {
-      const float n = fmaxf(m, rm), ref = n == -INFINITY ? 0.f : n;
-      z *= exp2_fast((m - ref) * c);
-#pragma unroll
-      for (int i = 0; i < kLaneCols; ++i) z += exp2_fast((r.v[i] - ref) * c);
-      m = n;
+  const int first = part * kWaves + wave, waves = g.split * kWaves;
+  if (a.open) {
+    const bool use_table = kTable && a.temp >= 0.5;
+    if constexpr (kTable) {
+      if (use_table) fill_table(table, [&](float v) { return exp2_product((double)v, a.k); });
     }
+    // m: this lane's maximum in the run, and (without the table) the logit whose mass is 1
+    float m = -INFINITY;
+    double mass = 0.0;
+    auto by_polynomial = [&](const Pack<T, VEC>& p, int) {
+      float v[VEC], n = m;
+      unpack(p, v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) n = fmaxf(n, v[i]);
+      const double ref = n == -INFINITY ? 0.0 : (double)n;
+      if (__any(n > m) && mass > 0.0) mass *= exp2_product((double)m - ref, a.k);
+      m = n;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) mass += exp2_product((double)v[i] - ref, a.k);
+    };
+    auto finish = [&](int run, bool table_done) {
+      const float rm = wave_max(m);
+      float ref = rm == -INFINITY ? 0.f : rm;
+      if (table_done) ref = 0.f;
+      else if (m != -INFINITY) mass *= exp2_product((double)m - (double)ref, a.k);
+      mass = wave_total(mass);
+      if (lane == 0) {
+        g.run_mass[row * g.runs + run] = mass;
+        g.run_max[row * g.runs + run] = rm;
+        g.run_ref[row * g.runs + run] = ref;
+      }
+      m = -INFINITY;
+      mass = 0.0;
+    };
+    if constexpr (kTable) {
+      if (use_table) {
+        each_run(
+            x, g.cols, g.runs, first, waves,
+            [&](const Pack<T, VEC>& p, int c) {
+              float v[VEC];
+              unpack(p, v);
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) m = fmaxf(m, v[i]);
+              // (a logit of 2^8 or more in size may take this sum out of range; the run is then done again)
+              mass += sum_table(table, p, x, c, g.cols, Bins<T>::kUsed,
+                                [&](float y) { return exp2_product((double)y, a.k); });
+            },
+            [&](int run) {
+              const float rm = wave_max(m);
+              if (fabsf(rm) >= 0x1p8f) {
+                m = -INFINITY;
+                mass = 0.0;
+                each_run(x, g.cols, run + 1, run, 1, by_polynomial, [](int) {});
+                finish(run, false);
+              } else {
+                finish(run, true);
+              }
+            });
+        return;
+      }
+    }
+    each_run(x, g.cols, g.runs, first, waves, by_polynomial, [&](int run) { finish(run, false); });
+    return;
   }
-  if (a.open) return;
-  z = wave_sum(z);
+  const float c = (float)a.k;
+  float m = -INFINITY, z = 0.f, rm = -INFINITY;  // rm: of the run
+  each_run(
+      x, g.cols, g.runs, first, waves,
+      [&](const Pack<T, VEC>& p, int) {
+        float v[VEC], q = v[0];
+        unpack(p, v);
+        q = v[0];
+#pragma unroll
+        for (int i = 1; i < VEC; ++i) q = fmaxf(q, v[i]);
+        rm = fmaxf(rm, q);
+        const float n = fmaxf(m, q), ref = n == -INFINITY ? 0.f : n;
+        z *= exp2_fast((m - ref) * c);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z += exp2_fast((v[i] - ref) * c);
+        m = n;
+      },
+      [&](int run) {
+        if (!a.by_k) return;
+        float q = rm;
+        q = fmaxf(q, dpp_move<dpp::kXor1>(q, q));
+        q = fmaxf(q, dpp_move<dpp::kXor2>(q, q));
+        q = fmaxf(q, dpp_move<dpp::kHalfMirror>(q, q));
+        q = fmaxf(q, dpp_move<dpp::kMirror>(q, q));
+        if (lane % 16 == 0) g.quarters[(row * g.runs + run) * 4 + lane / 16] = q;
+        rm = -INFINITY;
+      });
+  {
+    const float wm = wave_max(m), ref = wm == -INFINITY ? 0.f : wm;
+    z = wave_sum(m == -INFINITY ? z : z * exp2_fast((m - ref) * c));
+    m = wm;
+  }
   if (lane == 0) sm[wave] = m, sz[wave] = z;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < kWaves; ++i) m = fmaxf(m, sm[i]);
-    z = 0.f;
-    for (int i = 0; i < kWaves; ++i) z += sm[i] == -INFINITY ? sz[i] : sz[i] * exp2_fast((sm[i] - m) * c);
-    g.part_max[blockIdx.x] = m;
-    g.part_sum[blockIdx.x] = z;
-  }
+  if (wave > 0) return;
+  m = lane < kWaves ? sm[lane] : -INFINITY;
+  z = lane < kWaves ? sz[lane] : 0.f;
+  const float bm = wave_max(m);
+  z = wave_sum(m == -INFINITY ? z : z * exp2_fast((m - bm) * c));
+  if (lane == 0) g.part_max[blockIdx.x] = bm, g.part_sum[blockIdx.x] = z;
 }
 
 // ---- hist and cut -----------------------------------------------------------
 struct Fine {
-  u64 mass[kBins];
-  uint32_t count[kBins], key[kBins];
+  u64 mass[kFineBins];
+  uint32_t count[kFineBins], key[kFineBins];
 };
 // What the bins of a block's columns need, and what finding a cut needs beside.
-struct HistShared {
-  Hist linear;
-  float quarters[kMaxQuarters];
-  float bound;
+template <typename T> struct HistShared {
+  Hist<T> hist;
+  float least;
 };
-struct CutShared : HistShared {
+template <typename T> struct CutShared : HistShared<T> {
   Fine fine;
   u64 ltmp[kWaves];
   uint32_t utmp[kWaves];
@@ -322,132 +524,252 @@ struct CutShared : HistShared {
   u64 mass_before;
 };
 
-// The bin whose running count passes `count_target` (by count), or whose running mass reaches `mass_target`; what lies
-// before it goes to sh. Exactly one bin qualifies. Begins and ends with a barrier.
-__device__ __forceinline__ void find_bin(const u64* mass, const uint32_t* count, CutShared& sh, bool by_count,
-                                         uint32_t count_target, u64 mass_target) {
-  constexpr int kEach = kBins / kLanes;
-  __syncthreads();
-  if (threadIdx.x == 0) sh.bin = kBins - 1, sh.cnt_before = 0, sh.mass_before = 0;
-  const int b = kEach * threadIdx.x;
-  uint32_t c[kEach], cs = 0;
-  u64 m[kEach], ms = 0;
+// A thread's share of `BINS` bins: their counts and masses, and those of the bins before them.
+template <int BINS>
+struct Share {
+  static constexpr int kEach = BINS / kLanes;
+  static_assert(BINS % kLanes == 0, "whole turns");
+  uint32_t count[kEach], total, before;
+  u64 mass[kEach], mass_total, mass_before;
+  // (begins with a barrier)
+  template <typename S, typename M>
+  __device__ __forceinline__ Share(const uint32_t* counts, M&& mass_of, S& sh) : total(0), mass_total(0) {
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) c[i] = count[b + i], m[i] = mass[b + i], cs += c[i], ms += m[i];
-  uint32_t cb = block_before<uint32_t>(cs, sh.utmp);
-  u64 mb = block_before<u64>(ms, sh.ltmp);
+    for (int i = 0; i < kEach; ++i) count[i] = counts[kEach * threadIdx.x + i], total += count[i];
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const bool here = by_count ? cb < count_target && count_target - cb <= c[i]
-                               : mb < mass_target && mass_target - mb <= m[i];
-    if (here) sh.bin = b + i, sh.cnt_before = cb, sh.mass_before = mb;
-    cb += c[i];
-    mb += m[i];
+    for (int i = 0; i < kEach; ++i)
+      mass[i] = count[i] ? mass_of(kEach * (int)threadIdx.x + i, count[i]) : 0, mass_total += mass[i];
+    before = block_before<uint32_t>(total, sh.utmp);
+    mass_before = block_before<u64>(mass_total, sh.ltmp);
   }
-  __syncthreads();
-}
+  // The bin whose running count reaches `count_target` (by count), or whose running mass reaches `mass_target`; what
+  // lies before it goes to sh. Exactly one bin qualifies. Begins and ends with a barrier.
+  template <typename S>
+  __device__ __forceinline__ void find(S& sh, bool by_count, uint32_t count_target, u64 mass_target) const {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.bin = BINS - 1, sh.cnt_before = 0, sh.mass_before = 0;
+    __syncthreads();
+    uint32_t cb = before;
+    u64 mb = mass_before;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (by_count ? cb < count_target && count_target - cb <= count[i] : mb < mass_target && mass_target - mb <= mass[i])
+        sh.bin = kEach * threadIdx.x + i, sh.cnt_before = cb, sh.mass_before = mb;
+      cb += count[i];
+      mb += mass[i];
+    }
+    __syncthreads();
+  }
+};
 
 template <typename T>
 struct Row {
+  static constexpr int VEC = 16 / sizeof(T);
+  typedef Bins<T> B;
   const T* x;
   int cols, runs;
   float max;        // of the row
-  double to_log2;   // log2(e) / T
-  float bin_step;   // kBins / (kRange T)
+  double k;         // log2(e) / T
+  float bin_step;   // linear bins: bins / (kRange T)
   double magic;
 
-  __device__ __forceinline__ double mass(float v) const { return exp2_product((double)v - (double)max, to_log2); }
+  __device__ __forceinline__ Row(const SampleArgs& g, int64_t row, const Start& st)
+      : x(static_cast<const T*>(g.logits) + row * g.ld),
+        cols(g.cols),
+        runs(g.runs),
+        max(st.max),
+        k(st.a.k),
+        bin_step((float)(B::kCount / kRange * kLn2D * st.a.k)),
+        magic(g.magic) {}
+  __device__ __forceinline__ double mass(float v) const { return exp2_product((double)v - (double)max, k); }
   __device__ __forceinline__ u64 fixed(double e) const {
     return __builtin_bit_cast(u64, e + magic) & 0xfffffffffffffull;
   }
   __device__ __forceinline__ int bin_of(float v) const {
-    const float d = (max - v) * bin_step;
-    return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+    if constexpr (B::kExact) {
+      return B::of(v);
+    } else {
+      const float d = (max - v) * bin_step;
+      return d < (float)(B::kCount - 1) ? (int)d : B::kCount - 1;
+    }
+  }
+  __device__ __forceinline__ u64 mass_of_bin(const Hist<T>& h, int bin, uint32_t count) const {
+    if constexpr (B::kExact) {
+      if (B::several(bin)) return h.mass[B::slot(bin)];
+      return count * fixed(mass(B::value(bin)));
+    } else {
+      return h.mass[bin];
+    }
   }
 
-  // Adds the runs of one block (part of split) to sh.linear; logits below `least` are left out.
-  __device__ __forceinline__ void fill_linear(HistShared& sh, int part, int split, float least, bool masses) const {
-    for (int i = threadIdx.x; i < kBins; i += kLanes) sh.linear.mass[i] = 0, sh.linear.count[i] = 0;
+  // Adds the runs of one block (part of split) to h; logits below `least` are left out.
+  __device__ __forceinline__ void fill(Hist<T>& h, int part, int split, float least, bool masses) const {
+    for (int i = threadIdx.x; i < B::kCount; i += kLanes) h.count[i] = 0;
+    for (int i = threadIdx.x; i < B::kMasses; i += kLanes) h.mass[i] = 0;
     __syncthreads();
-    uint32_t low = 0;
+    uint32_t low = 0;  // of the last bin, which masked tokens and most of a peaked row share
     u64 low_mass = 0;
-    for (int run = part * kWaves + (int)threadIdx.x / kWave; run < runs; run += split * kWaves) {
-      Run<T> r;
-      r.load(x, run, cols);
+    const int first = part * kWaves + (int)threadIdx.x / kWave, waves = split * kWaves;
+    if constexpr (B::kExact) {
+      constexpr int kLow = Bins<__bf16>::kUsed - 1;
+      // (what is left out counts as low: the k-th logit lies above)
+      const int reach = least == -INFINITY ? kLow - 1 : ::min(kLow - 1, B::of(least));
+      each_run(
+          x, cols, runs, first, waves,
+          [&](const Pack<T, VEC>& p, int c) {
+            typename B::Two low2 = (typename B::Two)((short)B::kSide), high2 = (typename B::Two)((short)0);
 #pragma unroll
-      for (int i = 0; i < kLaneCols; ++i) {
-        if (r.v[i] >= least) {
-          const int b = bin_of(r.v[i]);
-          const u64 e = masses ? fixed(mass(r.v[i])) : 0;
-          if (b < kBins - 1) {
-            atomicAdd(&sh.linear.count[b], 1u);
-            if (masses) atomicAdd(&sh.linear.mass[b], e);
-          } else {
-            ++low;
-            low_mass += e;
-          }
+            for (int j = 0; j < 4; ++j) {
+              typename B::Two rank;
+              const typename B::Two b = B::of_two(p.w[j], &rank);
+              low2 = __builtin_elementwise_min(low2, rank);
+              high2 = __builtin_elementwise_max(high2, rank);
+              if (b.x <= reach) atomicAdd(&h.count[b.x], 1u);
+              else ++low;
+              if (b.y <= reach) atomicAdd(&h.count[b.y], 1u);
+              else ++low;
+            }
+            if (masses && (::min(low2.x, low2.y) == 0 || ::max(high2.x, high2.y) > B::kSide)) {
+#pragma unroll 1
+              for (int i = c; i < ::min(c + VEC, cols); ++i) {
+                const float v = to_f32<T>(x[i]);
+                const int b = B::of(v);
+                if (B::several(b) && v != -INFINITY) atomicAdd(&h.mass[B::slot(b)], fixed(mass(v)));
+              }
+            }
+          },
+          [](int) {});
+      low = wave_total(low);
+      if (threadIdx.x % kWave == 0) atomicAdd(&h.count[kLow], low);
+    } else {
+      constexpr int kLow = B::kCount - 1;
+      each_run(
+          x, cols, runs, first, waves,
+          [&](const Pack<T, VEC>& p, int) {
+            float v[VEC];
+            unpack(p, v);
+            float most = v[0];
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
+            if (!__any(most >= least)) return;
+            u64 e[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) e[i] = 0;
+            if (masses) {
+#pragma unroll
+              for (int i = 0; i < VEC; ++i) e[i] = fixed(mass(v[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const int b = bin_of(v[i]);
+              if (v[i] >= least && b < kLow) {
+                atomicAdd(&h.count[b], 1u);
+                if (masses) atomicAdd(&h.mass[b], e[i]);
+              } else {
+                ++low;  // (what is left out counts as low: the k-th logit lies above)
+                low_mass += e[i];
+              }
+            }
+          },
+          [](int) {});
+      low = wave_total(low);
+      low_mass = wave_total(low_mass);
+      if (threadIdx.x % kWave == 0) {
+        atomicAdd(&h.count[kLow], low);
+        if (masses) atomicAdd(&h.mass[kLow], low_mass);
+      }
+    }
+  }
+
+  // The values that a bin can hold, as a range of keys; true (and the value) if there is one only.
+  __device__ __forceinline__ bool one_value(int bin, uint32_t* klo, uint32_t* khi, float* value) const {
+    if constexpr (B::kExact) {
+      if (!B::several(bin)) {
+        *value = B::value(bin);
+        return true;
+      }
+      *khi = bin == 0 ? key_of<T>(max) : bin == B::kZero ? key_of<T>(0x1p-12f) : key_of<T>(-0x1p8f);
+      *klo = bin == 0 ? key_of<T>(0x1p8f) : bin == B::kZero ? key_of<T>(-0x1p-12f) : 0;
+      return false;
+    } else {
+      // with the roundings of bin_of to spare
+      const double width = 1.0 / (double)bin_step, slack = 0x1p-21;
+      const float hi = (float)((double)max - bin * width * (1 - slack));
+      const float lo = (float)((double)max - (bin + 1) * width * (1 + slack));
+      *khi = bin == 0 ? key_of<T>(max) : ::min(key_of<T>(max), key_of<T>(hi) + 1);
+      const uint32_t kl = key_of<T>(lo);
+      *klo = bin == B::kCount - 1 || kl == 0 ? 0 : kl - 1;
+      int values = 0;
+      if (*khi - *klo < 16) {
+#pragma unroll 1
+        for (uint32_t key = *klo; key <= *khi; ++key) {
+          const float v = value_of<T>(key);
+          if (bin_of(v) == bin) ++values, *value = v;
         }
       }
-    }
-    low = wave_total(low);
-    low_mass = wave_total(low_mass);
-    if (threadIdx.x % kWave == 0) {
-      atomicAdd(&sh.linear.count[kBins - 1], low);
-      if (masses) atomicAdd(&sh.linear.mass[kBins - 1], low_mass);
+      return values == 1;
     }
   }
 
-  // The cut after `k` logits (by count) or at mass `tau` (fixed point), and the mass that it keeps.
-  __device__ __forceinline__ Cut find_cut(CutShared& sh, bool by_count, uint32_t k, u64 tau, bool masses,
-                                          u64* kept) const {
-    find_bin(sh.linear.mass, sh.linear.count, sh, by_count, k, tau);
-    const int lin = sh.bin;
+  // The cut after `count` logits (by count) or at mass `tau` (fixed point), and the mass that it keeps.
+  __device__ __forceinline__ Cut find_cut(CutShared<T>& sh, const Share<B::kCount>& share, bool by_count, uint32_t count,
+                                          u64 tau, bool masses, u64* kept) const {
+    share.find(sh, by_count, count, tau);
+    const int bin = sh.bin;
     uint32_t cnt = sh.cnt_before;
     u64 above = sh.mass_before;
-    // keys that the bin can hold, with the roundings of bin_of to spare
-    const double width = 1.0 / (double)bin_step, slack = 0x1p-21;
-    const float hi = (float)((double)max - lin * width * (1 - slack));
-    const float lo = (float)((double)max - (lin + 1) * width * (1 + slack));
-    uint32_t khi = lin == 0 ? key_of<T>(max) : ::min(key_of<T>(max), key_of<T>(hi) + 1);
-    const uint32_t kl = key_of<T>(lo);
-    uint32_t klo = lin == kBins - 1 || kl == 0 ? 0 : kl - 1;
+    uint32_t klo, khi;
     float value = max;
     uint32_t equal = 0;
-    // one value of T in the bin (16-bit logits away from 0): nothing to look at
-    int values = 0;
-    if (khi - klo < 16) {
-      for (uint32_t key = klo; key <= khi; ++key) {
-        const float v = value_of<T>(key);
-        if (bin_of(v) == lin) ++values, value = v;
-      }
-    }
-    if (values == 1) {
-      equal = sh.linear.count[lin];
+    if (one_value(bin, &klo, &khi, &value)) {
+      equal = sh.hist.count[bin];
     } else {
       // 32 bits of key in turns of 11
+#pragma unroll 1
       for (int turn = 0; turn < 3; ++turn) {
         int s = 0;
-        while (((khi - klo) >> s) >= (uint32_t)kBins) ++s;
+        while (((khi - klo) >> s) >= (uint32_t)kFineBins) ++s;
         __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kLanes) sh.fine.mass[i] = 0, sh.fine.count[i] = 0, sh.fine.key[i] = 0;
+        for (int i = threadIdx.x; i < kFineBins; i += kLanes) sh.fine.mass[i] = 0, sh.fine.count[i] = 0, sh.fine.key[i] = 0;
         __syncthreads();
-        for (int run = threadIdx.x / kWave; run < runs; run += kWaves) {
-          Run<T> r;
-          r.load(x, run, cols);
+        // one block reads the row: it needs many loads on their way, and finds few logits
+        constexpr int kAhead = 6, kStep = kLanes * VEC;
+#pragma unroll 1
+        for (int c0 = (int)threadIdx.x * VEC; c0 < cols; c0 += kAhead * kStep) {
+          Pack<T, VEC> p[kAhead];
 #pragma unroll
-          for (int i = 0; i < kLaneCols; ++i) {
-            if (bin_of(r.v[i]) == lin) {
-              const uint32_t key = key_of<T>(r.v[i]);
-              if (key >= klo && key <= khi) {
+          for (int j = 0; j < kAhead; ++j)
+            if (c0 + j * kStep + VEC <= cols) p[j] = load_pack_any<T, VEC>(x + c0 + j * kStep);
+          uint32_t some = 0;
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) {
+            float v[VEC];
+            unpack(p[j], v);
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) any = any || bin_of(v[i]) == bin;
+            // (the columns of a vector that reaches past the row are looked at below)
+            if (c0 + j * kStep + VEC <= cols ? any : c0 + j * kStep < cols) some |= 1u << j;
+          }
+#pragma unroll 1
+          for (; some; some &= some - 1) {
+            const int c = c0 + __builtin_ctz(some) * kStep;
+#pragma unroll 1
+            for (int i = c; i < ::min(c + VEC, cols); ++i) {
+              const float y = to_f32<T>(x[i]);
+              const uint32_t key = key_of<T>(y);
+              if (bin_of(y) == bin && key >= klo && key <= khi) {
                 const uint32_t b = (khi - key) >> s;
                 atomicAdd(&sh.fine.count[b], 1u);
                 atomicMax(&sh.fine.key[b], key);
-                if (masses) atomicAdd(&sh.fine.mass[b], fixed(mass(r.v[i])));
+                if (masses) atomicAdd(&sh.fine.mass[b], fixed(mass(y)));
               }
             }
           }
         }
-        find_bin(sh.fine.mass, sh.fine.count, sh, by_count, k - cnt, tau - above);
+        const Share<kFineBins> fine(sh.fine.count, [&](int b, uint32_t) { return sh.fine.mass[b]; }, sh);
+        fine.find(sh, by_count, count - cnt, tau - above);
         const uint32_t b = (uint32_t)sh.bin;
         cnt += sh.cnt_before;
         above += sh.mass_before;
@@ -463,242 +785,249 @@ struct Row {
     cut.equal = equal;
     const u64 each = masses ? fixed(mass(value)) : 0;
     // (by mass: the bin holds equal * each >= tau - above > 0)
-    cut.ties = by_count ? k - cnt : (uint32_t)((tau - above + each - 1) / each);
+    cut.ties = by_count ? count - cnt : (uint32_t)((tau - above + each - 1) / each);
     *kept = above + each * cut.ties;
     return cut;
   }
 
-  // The row's cut by top-k and top-p, from sh.linear.
-  __device__ __forceinline__ Cut find(CutShared& sh, const Asked& a) const {
-    Cut cut = {-INFINITY, 0xffffffffu, 0};
-    u64 total = 0;
-    if (a.by_k) cut = find_cut(sh, true, (uint32_t)a.top_k, 0, a.by_p, &total);
-    if (a.by_p) {
-      if (!a.by_k) {
-        __syncthreads();
-        u64 t = 0;
-        for (int i = threadIdx.x; i < kBins; i += kLanes) t += sh.linear.mass[i];
-        t = wave_total(t);
-        if (threadIdx.x % kWave == 0) sh.ltmp[threadIdx.x / kWave] = t;
-        __syncthreads();
-        for (int i = 0; i < kWaves; ++i) total += sh.ltmp[i];
-      }
+  // The row's cut by top-k and top-p, from sh.hist.
+  __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a) const {
+    const Share<B::kCount> share(
+        sh.hist.count, [&](int b, uint32_t c) { return a.by_p ? mass_of_bin(sh.hist, b, c) : 0; }, sh);
+    u64 total = total_of(sh.ltmp);
+    Cut cut = {INFINITY, 0, 0};
+    // by count, then by mass of what that kept
+#pragma unroll 1
+    for (int turn = a.by_k ? 0 : 1; turn < (a.by_p ? 2 : 1); ++turn) {
       const u64 tau = ::min(total, ::max((u64)1, (u64)ceil(fmax(a.top_p, 0.0) * (double)total)));
-      u64 unused;
-      const Cut p = find_cut(sh, false, 0, tau, true, &unused);
-      if (!a.by_k || p.x > cut.x) cut = p;
-      else if (p.x == cut.x && p.ties < cut.ties) cut.ties = p.ties;
+      u64 kept;
+      const Cut c = find_cut(sh, share, turn == 0, (uint32_t)a.top_k, tau, a.by_p, &kept);
+      if (turn == 0 || !a.by_k || c.x > cut.x) cut = c;
+      else if (c.x == cut.x && c.ties < cut.ties) cut.ties = c.ties;
+      total = kept;
     }
     return cut;
   }
 };
 
-template <typename T>
-__device__ __forceinline__ Row<T> row_of(const SampleArgs& g, int64_t row, const Asked& a, float max) {
-  Row<T> r;
-  r.x = static_cast<const T*>(g.logits) + row * g.ld;
-  r.cols = g.cols;
-  r.runs = g.runs;
-  r.max = max;
-  r.to_log2 = 1.4426950408889634074 / a.temp;
-  r.bin_step = (float)(kBins / (kRange * a.temp));
-  r.magic = g.magic;
-  return r;
-}
-
 // A lower bound of the k-th largest logit: the k-th largest of the maxima of 512 columns (each of those k is a logit of
-// its own), where there are enough of them.
-__device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row, const Asked& a, HistShared& sh) {
+// its own) to 16 bits of key, where there are enough of them. The first wave finds it, bit by bit.
+__device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row, const Asked& a, float* shared) {
+  constexpr int kMost = kMaxQuarters / kWave;
   const int n = 4 * g.runs;
   if (!a.by_k || a.top_k > n || n > kMaxQuarters) return -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kLanes) sh.quarters[i] = g.quarters[row * n + i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kLanes) {
-    const float v = sh.quarters[i];
-    int before = 0;
-    for (int j = 0; j < n; ++j) before += sh.quarters[j] > v || (sh.quarters[j] == v && j < i);
-    if (before == (int)a.top_k - 1) sh.bound = v;
+  if (threadIdx.x < kWave) {
+    uint32_t key[kMost];
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) {
+      const int i = j * kWave + (int)threadIdx.x;
+      key[j] = i < n ? key_of<__bf16>(g.quarters[row * n + i]) : 0;
+    }
+    uint32_t least = 0;
+#pragma unroll 1
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t tried = least | 1u << bit;
+      int count = 0;
+#pragma unroll
+      for (int j = 0; j < kMost; ++j)
+        if (j * kWave < n) count += __popcll(__ballot(key[j] >= tried));
+      if (count >= (int)a.top_k) least = tried;
+    }
+    // (0x7f: -inf)
+    if (threadIdx.x == 0)
+      *shared = least <= 0x7f ? -INFINITY : bits_f32((least & 0x8000u) ? (least ^ 0x8000u) << 16 : ~(least << 16));
   }
   __syncthreads();
-  return sh.bound;
+  return *shared;
 }
 
 // WHOLE: one block has the whole row (split 1) and goes on to the cut.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
-  __shared__ typename std::conditional<WHOLE, CutShared, HistShared>::type sh;
+  __shared__ typename std::conditional<WHOLE, CutShared<T>, HistShared<T>>::type sh;
   const int64_t row = blockIdx.x / g.split;
-  const Asked a = asked(g, row);
-  if (!a.by_k && !a.by_p) return;
-  float max, sum;
-  if (!row_state(g, row, a, &max, &sum)) return;
-  const Row<T> r = row_of<T>(g, row, a, max);
-  r.fill_linear(sh, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, a, sh), a.by_p);
+  const Start st(g, row, false);
+  if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
+  const Row<T> r(g, row, st);
+  r.fill(sh.hist, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, st.a, &sh.least), st.a.by_p);
   if constexpr (WHOLE) {
-    const Cut cut = r.find(sh, a);
+    const Cut cut = r.find(sh, st.a);
     if (threadIdx.x == 0) g.cuts[row] = cut;
   } else {
     __syncthreads();
-    Hist& to = g.hist[blockIdx.x];
-    for (int i = threadIdx.x; i < kBins; i += kLanes) {
-      to.count[i] = sh.linear.count[i];
-      if (a.by_p) to.mass[i] = sh.linear.mass[i];
-    }
+    Hist<T>& to = static_cast<Hist<T>*>(g.hist)[blockIdx.x];
+    for (int i = threadIdx.x; i < Bins<T>::kCount; i += kLanes) to.count[i] = sh.hist.count[i];
+    if (st.a.by_p)
+      for (int i = threadIdx.x; i < Bins<T>::kMasses; i += kLanes) to.mass[i] = sh.hist.mass[i];
   }
+}
+
+// Element i of the `split` arrays that lie `stride` bytes apart, added up; the loads are in flight together.
+template <typename V>
+__device__ __forceinline__ V sum_parts(const char* p, size_t stride, int split) {
+  V v[kMaxSplit], sum = {};
+#pragma unroll
+  for (int i = 0; i < kMaxSplit; ++i)
+    if (i < split) v[i] = *reinterpret_cast<const V*>(p + i * stride);
+#pragma unroll
+  for (int i = 0; i < kMaxSplit; ++i)
+    if (i < split) sum += v[i];
+  return sum;
 }
 
 // (split > 1)
 template <typename T>
 __global__ __launch_bounds__(kLanes) void sample_cut_kernel(SampleArgs g) {
-  __shared__ CutShared sh;
+  typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+  __shared__ __align__(16) CutShared<T> sh;
   const int64_t row = blockIdx.x;
-  const Asked a = asked(g, row);
-  if (!a.by_k && !a.by_p) return;
-  float max, sum;
-  if (!row_state(g, row, a, &max, &sum)) return;
-  const Row<T> r = row_of<T>(g, row, a, max);
-  const Hist* from = g.hist + row * g.split;
-  for (int i = threadIdx.x; i < kBins; i += kLanes) {
-    uint32_t c = 0;
-    u64 m = 0;
-    for (int p = 0; p < g.split; ++p) {
-      c += from[p].count[i];
-      if (a.by_p) m += from[p].mass[i];
-    }
-    sh.linear.count[i] = c;
-    sh.linear.mass[i] = m;
-  }
-  const Cut cut = r.find(sh, a);
+  const Start st(g, row, false);
+  if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
+  const Row<T> r(g, row, st);
+  const Hist<T>* from = static_cast<const Hist<T>*>(g.hist) + row * g.split;
+#pragma unroll 1
+  for (int i = 4 * threadIdx.x; i < Bins<T>::kCount; i += 4 * kLanes)
+    *reinterpret_cast<u32x4*>(&sh.hist.count[i]) = sum_parts<u32x4>((const char*)&from->count[i], sizeof(Hist<T>), g.split);
+  if (st.a.by_p)
+#pragma unroll 1
+    for (int i = 2 * threadIdx.x; i < Bins<T>::kMasses; i += 2 * kLanes)
+      *reinterpret_cast<u64x2*>(&sh.hist.mass[i]) =
+          sum_parts<u64x2>((const char*)&from->mass[i], sizeof(Hist<T>), g.split);
+  const Cut cut = r.find(sh, st.a);
   if (threadIdx.x == 0) g.cuts[row] = cut;
-}
-
-// The row's cut with min-p in it.
-__device__ __forceinline__ Cut final_cut(const SampleArgs& g, int64_t row, const Asked& a, float max) {
-  Cut cut = {-INFINITY, 0xffffffffu, 0};
-  if (a.by_k || a.by_p) cut = g.cuts[row];
-  if (a.min_p > 0.0) {
-    // e^((x - max) / T) >= min_p, as the smallest float that satisfies it
-    const double least = (double)max + a.temp * log(fmin(a.min_p, 1.0));
-    float f = (float)least;
-    if ((double)f < least) f = nextafterf(f, INFINITY);
-    if (f > cut.x) cut = {f, 0xffffffffu, 0};
-  }
-  return cut;
 }
 
 // ---- mass -------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr bool kTable = Bins<T>::kExact;
+  __shared__ double table[kTable ? Bins<__bf16>::kUsed : 1];
   const int64_t row = blockIdx.x / g.split;
   const int part = blockIdx.x % g.split;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const Asked a = asked(g, row);
-  if (a.open) return;
-  float max, sum;
-  if (!row_state(g, row, a, &max, &sum)) return;
-  const Cut cut = final_cut(g, row, a, max);
-  const Row<T> r = row_of<T>(g, row, a, max);
+  const Start st(g, row, true);
+  if (!st.ok || st.a.open) return;
+  const Row<T> r(g, row, st);
+  const Cut cut = st.cut;
   const bool all_ties = cut.ties >= cut.equal;
-  for (int run = part * kWaves + wave; run < g.runs; run += g.split * kWaves) {
-    Run<T> l;
-    l.load(r.x, run, g.cols);
-    double mass = 0.0;
-    uint32_t ties = 0;
-#pragma unroll
-    for (int i = 0; i < kLaneCols; ++i) {
-      const float v = l.v[i];
-      if (v >= cut.x) {
-        if (all_ties || v > cut.x) mass += r.mass(v);
-        else ++ties;
-      }
-    }
-    mass = wave_total(mass);
-    ties = wave_total(ties);
-    if (lane == 0) g.run_mass[row * g.runs + run] = mass, g.run_ties[row * g.runs + run] = ties;
+  auto kept = [&](float v) { return all_ties ? v >= cut.x : v > cut.x; };
+  int reach = 0;
+  if constexpr (kTable) {
+    fill_table(table, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
+    reach = Bins<T>::of(cut.x);
   }
+  double mass = 0.0;
+  uint32_t ties = 0;
+  each_run(
+      r.x, g.cols, g.runs, part * kWaves + wave, g.split * kWaves,
+      [&](const Pack<T, VEC>& p, int c) {
+        float v[VEC];
+        unpack(p, v);
+        if constexpr (kTable) {
+          mass += sum_table(table, p, r.x, c, g.cols, reach, [&](float y) { return kept(y) ? r.mass(y) : 0.0; });
+        } else {
+          float most = v[0];
+#pragma unroll
+          for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
+          if (__any(most >= cut.x)) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) mass += kept(v[i]) ? r.mass(v[i]) : 0.0;
+          }
+        }
+        if (!all_ties) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) ties += v[i] == cut.x ? 1 : 0;
+        }
+      },
+      [&](int run) {
+        mass = wave_total(mass);
+        ties = wave_total(ties);
+        if (lane == 0) g.run_mass[row * g.runs + run] = mass, g.run_ties[row * g.runs + run] = ties;
+        mass = 0.0;
+        ties = 0;
+      });
 }
 
 // ---- pick -------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(kPickLanes) void sample_pick_kernel(SampleArgs g) {
-  constexpr int kPickWaves = kPickLanes / kWave;
-  constexpr int kCols = kRun / kPickLanes;  // columns a thread, in order
-  __shared__ double dtmp[kPickWaves];
-  __shared__ uint32_t utmp[kPickWaves];
-  __shared__ float ftmp[kPickWaves];
-  __shared__ int found, last, sh_run;
+__global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
+  constexpr int kCols = kRun / kLanes;  // columns a thread, in order
+  __shared__ double dtmp[kWaves];
+  __shared__ uint32_t utmp[kWaves];
+  __shared__ float ftmp[kWaves];
+  __shared__ int itmp[2 * kWaves], sh_run;
   __shared__ double sh_base;
   __shared__ uint32_t sh_ties;
   const int64_t row = blockIdx.x;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const Asked a = asked(g, row);
   const double* run_mass = g.run_mass + row * g.runs;
   const uint32_t* run_ties = g.run_ties + row * g.runs;
-  const float* run_max = g.run_max + row * g.runs;
-  const int per = (g.runs + kPickLanes - 1) / kPickLanes;  // runs a thread, in order
+  const float *run_max = g.run_max + row * g.runs, *run_ref = g.run_ref + row * g.runs;
+  const int per = (g.runs + kLanes - 1) / kLanes;  // runs a thread, in order
   const int r0 = min(g.runs, (int)threadIdx.x * per), r1 = min(g.runs, r0 + per);
+  // the first run's records, on the way while the row's start is put together (mostly there is no other)
+  const int any_run = min(r0, g.runs - 1);
+  const double mass0 = run_mass[any_run];
+  const uint32_t ties0 = run_ties[any_run];
+  const float max0 = run_max[any_run], ref0 = run_ref[any_run];
+  Start st(g, row, true);
+  const Asked& a = st.a;
+  const float u = g.u[row];
 
-  float max, sum = 0.f;
   bool fine = a.in_range;
   if (a.open) {
     float m = -INFINITY;
-    for (int i = r0; i < r1; ++i) m = fmaxf(m, run_max[i]);
+    for (int i = r0; i < r1; ++i) m = fmaxf(m, i == r0 ? max0 : run_max[i]);
     m = wave_max(m);
     if (lane == 0) ftmp[wave] = m;
     __syncthreads();
-    max = ftmp[0];
-    for (int i = 1; i < kPickWaves; ++i) max = fmaxf(max, ftmp[i]);
+    st.max = ftmp[0];
+    for (int i = 1; i < kWaves; ++i) st.max = fmaxf(st.max, ftmp[i]);
   } else {
-    fine = row_state(g, row, a, &max, &sum);
+    fine = st.ok;
   }
   if (!fine) {
     if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
     return;
   }
-  const Row<T> r = row_of<T>(g, row, a, max);
-  const Cut cut = a.open ? Cut{-INFINITY, 0xffffffffu, 0} : final_cut(g, row, a, max);
+  const float max = st.max;
+  const Row<T> r(g, row, st);
+  const Cut cut = a.open ? Cut{-INFINITY, 0xffffffffu, 0} : st.cut;
   const bool all_ties = cut.ties >= cut.equal;
   const double each = all_ties ? 0.0 : r.mass(cut.x);
 
-  // the masses of the runs: an open row's are relative to the run's own maximum
+  // the masses of the runs (an open row's in terms of their own reference)
   uint32_t ties = 0, seen = 0;
   if (!all_ties) {
-    for (int i = r0; i < r1; ++i) ties += run_ties[i];
+    for (int i = r0; i < r1; ++i) ties += i == r0 ? ties0 : run_ties[i];
     seen = block_before<uint32_t>(ties, utmp);
   }
   auto mass_of = [&](int i, uint32_t& ties_before) {
-    if (a.open) {
-      const float m = run_max[i];
-      return m == -INFINITY ? run_mass[i] : run_mass[i] * r.mass(m);
-    }
-    if (all_ties) return run_mass[i];
-    const uint32_t t = run_ties[i], left = cut.ties - min(cut.ties, ties_before);
+    const double m = i == r0 ? mass0 : run_mass[i];
+    if (a.open) return m * exp2_product((double)(i == r0 ? ref0 : run_ref[i]) - (double)max, r.k);
+    if (all_ties) return m;
+    const uint32_t t = i == r0 ? ties0 : run_ties[i], left = cut.ties - min(cut.ties, ties_before);
     ties_before += t;
-    return run_mass[i] + each * (double)min(left, t);
+    return m + each * (double)min(left, t);
   };
   double mass = 0.0;
   uint32_t rank = seen;
+#pragma unroll 1
   for (int i = r0; i < r1; ++i) mass += mass_of(i, rank);
   const double before = block_before<double>(mass, dtmp);
-  if (threadIdx.x == 0) found = kPickLanes, last = -1;
-  __syncthreads();
-  double total = 0.0;
-  for (int i = 0; i < kPickWaves; ++i) total += dtmp[i];
+  const double total = total_of(dtmp);
   if (!(total > 0.0 && total < INFINITY && max < INFINITY)) {  // (only an open row's can be)
     if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
     return;
   }
-  const double target = (double)g.u[row] * total;
+  const double target = (double)u * total;
   // the first thread that passes the target; if none does, the last one with any mass
-  if (mass > 0.0) {
-    if (before + mass > target) atomicMin(&found, (int)threadIdx.x);
-    atomicMax(&last, (int)threadIdx.x);
-  }
-  __syncthreads();
-  if ((int)threadIdx.x == (found < kPickLanes ? found : last)) {
+  if ((int)threadIdx.x == first_or_last(mass > 0.0 && before + mass > target, mass > 0.0, itmp)) {
     double s = before;
     int run = r0;
     rank = seen;
+#pragma unroll 1
     for (int i = r0; i < r1; ++i) {
       const uint32_t rank_before = rank;
       const double m = mass_of(i, rank);
@@ -731,14 +1060,7 @@ __global__ __launch_bounds__(kPickLanes) void sample_pick_kernel(SampleArgs g) {
     mass += e[i];
   }
   double s = base + block_before<double>(mass, dtmp);
-  if (threadIdx.x == 0) found = kPickLanes, last = -1;
-  __syncthreads();
-  if (mass > 0.0) {
-    if (s + mass > target) atomicMin(&found, (int)threadIdx.x);
-    atomicMax(&last, (int)threadIdx.x);
-  }
-  __syncthreads();
-  if ((int)threadIdx.x != (found < kPickLanes ? found : last)) return;
+  if ((int)threadIdx.x != first_or_last(mass > 0.0 && s + mass > target, mass > 0.0, itmp)) return;
   int id = -1;
   float at = 0.f;
   bool done = false;
@@ -749,19 +1071,19 @@ __global__ __launch_bounds__(kPickLanes) void sample_pick_kernel(SampleArgs g) {
     done = done || (e[i] > 0.0 && s > target);
   }
   g.ids[row] = id;
-  g.logp[row] = (float)(((double)at - (double)max) / a.temp) - log_fast(a.open ? (float)total : sum);
+  g.logp[row] = (float)(((double)at - (double)max) * r.k * kLn2D) - log_fast(a.open ? (float)total : st.sum);
 }
 
-// Blocks a row: enough for three blocks a CU, each with a run a wave at least.
+// Blocks a row: enough for two blocks a CU, each with a run a wave at least.
 int split_of(int64_t rows, int64_t runs, int64_t cus) {
-  const int64_t want = cdiv(3 * cus, std::max<int64_t>(rows, 1));
+  const int64_t want = cdiv(2 * cus, std::max<int64_t>(rows, 1));
   return (int)std::max<int64_t>(1, std::min<int64_t>({want, (int64_t)kMaxSplit, cdiv(runs, (int64_t)kWaves)}));
 }
 
 struct Layout {
-  size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, hist, cuts, total;
+  size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, run_ref, hist, cuts, total;
 };
-Layout layout_of(int64_t rows, int64_t runs, int64_t split, bool cuts) {
+Layout layout_of(int64_t rows, int64_t runs, int64_t split, bool cuts, bool bf16) {
   Layout l = {};
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -772,12 +1094,13 @@ Layout layout_of(int64_t rows, int64_t runs, int64_t split, bool cuts) {
   l.run_mass = take((size_t)(rows * runs) * sizeof(double));
   l.run_ties = take((size_t)(rows * runs) * sizeof(uint32_t));
   l.run_max = take((size_t)(rows * runs) * sizeof(float));
+  l.run_ref = take((size_t)(rows * runs) * sizeof(float));
   l.part_max = take((size_t)(rows * split) * sizeof(float));
   l.part_sum = take((size_t)(rows * split) * sizeof(float));
   if (cuts) {
     l.quarters = take((size_t)(rows * runs) * 4 * sizeof(float));
     l.cuts = take((size_t)rows * sizeof(Cut));
-    if (split > 1) l.hist = take((size_t)(rows * split) * sizeof(Hist));
+    if (split > 1) l.hist = take((size_t)(rows * split) * (bf16 ? sizeof(Hist<__bf16>) : sizeof(Hist<float>)));
   }
   l.total = at;
   return l;
@@ -790,11 +1113,11 @@ using namespace hk;
 
 extern "C" {
 
-size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int device) {
+size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int dtype, int device) {
   if (rows < 0 || rows >= (1LL << 31) || cols <= 0 || cols > (1 << 30)) return 0;
   const int cus = cu_count(device);
   const int64_t runs = cdiv(cols, (int64_t)kRun);
-  return std::max<size_t>(256, layout_of(rows, runs, split_of(rows, runs, cus > 0 ? cus : 256), cuts != 0).total);
+  return std::max<size_t>(256, layout_of(rows, runs, split_of(rows, runs, cus > 0 ? cus : 256), cuts != 0, dtype == kBF16).total);
 }
 
 int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int64_t rows, int64_t cols, int64_t ld,
@@ -823,7 +1146,7 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   HK_REQUIRE(rows * split < (1LL << 31), "rows=%lld too large", (long long)rows);
   const bool cuts = top_k_rows || (top_k > 0 && top_k < cols) || top_p_rows || top_p < 1;
   const bool masses = cuts || min_p_rows || min_p > 0;
-  const Layout l = layout_of(rows, runs, split, cuts);
+  const Layout l = layout_of(rows, runs, split, cuts, dtype == kBF16);
   HK_REQUIRE(workspace_bytes >= l.total, "workspace too small: need %zu bytes, got %zu", l.total, workspace_bytes);
   char* ws = (char*)workspace;
   SampleArgs g = {};
@@ -841,6 +1164,7 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   g.cols = (int)cols;
   g.runs = (int)runs;
   g.split = split;
+  g.has_cuts = cuts;
   int log2_cols = 0;
   while ((1LL << log2_cols) < cols + kRun) ++log2_cols;
   g.magic = (double)(1ULL << (52 - std::min(43, 63 - log2_cols)));
@@ -850,7 +1174,8 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   g.run_mass = (double*)(ws + l.run_mass);
   g.run_ties = (uint32_t*)(ws + l.run_ties);
   g.run_max = (float*)(ws + l.run_max);
-  g.hist = (Hist*)(ws + l.hist);
+  g.run_ref = (float*)(ws + l.run_ref);
+  g.hist = ws + l.hist;
   g.cuts = (Cut*)(ws + l.cuts);
   auto launch = [&](auto tag) {
     using T = decltype(tag);
@@ -871,7 +1196,7 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
       hipLaunchKernelGGL((sample_mass_kernel<T>), parts, dim3(kLanes), 0, st, g);
       if (const int rc = check_launch("sample_mass_kernel")) return rc;
     }
-    hipLaunchKernelGGL((sample_pick_kernel<T>), each, dim3(kPickLanes), 0, st, g);
+    hipLaunchKernelGGL((sample_pick_kernel<T>), each, dim3(kLanes), 0, st, g);
     return check_launch("sample_pick_kernel");
   };
   if (dtype == kF32) return launch(float{});

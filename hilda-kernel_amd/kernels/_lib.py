@@ -48,7 +48,7 @@ SIGNATURES = {
     "hk_rms_norm_quant_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _i32, _f32, _p]),
     "hk_sample": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _p, _f64, _p, _i32, _i64, _p, _f64, _p, _f64, _i32, _p, _sz,
                          _p]),
-    "hk_sample_workspace_size": (_sz, [_i64, _i64, _i32, _i32]),
+    "hk_sample_workspace_size": (_sz, [_i64, _i64, _i32, _i32, _i32]),
     "hk_swiglu_fwd": (_i32, [_p, _p, _p, _i64, _i32, _p]),
     "hk_swiglu_bwd": (_i32, [_p, _p, _p, _p, _p, _i64, _i32, _p]),
     "hk_geglu_fwd": (_i32, [_p, _p, _p, _i64, _i32, _p]),

@@ -66,13 +66,13 @@ def hilda_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     strides = logits.stride()
     if len(strides) != 2 or strides[1] != 1 or strides[0] < vocab:
         logits = logits.reshape(-1, vocab).contiguous()
-    rows = logits.shape[0]
+    rows, code = logits.shape[0], _lib.dtype_code(logits)
     ids = torch.empty(shape, dtype=torch.int64, device=dev)
     logp = torch.empty(shape, dtype=torch.float32, device=dev)
     cuts = k_rows is not None or p_rows is not None or 0 < k < vocab or p < 1
-    nbytes = _lib.load().hk_sample_workspace_size(rows, vocab, cuts, dev.index)
+    nbytes = _lib.load().hk_sample_workspace_size(rows, vocab, cuts, code, dev.index)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "hk_sample", ids.data_ptr(), logp.data_ptr(), logits.data_ptr(), uniform.data_ptr(), rows, vocab,
                  logits.stride(0) if rows > 1 else vocab, _lib.ptr(t_rows), t, _lib.ptr(k_rows), k_code, k,
-                 _lib.ptr(p_rows), p, _lib.ptr(m_rows), m, _lib.dtype_code(logits), ws.data_ptr(), nbytes)
+                 _lib.ptr(p_rows), p, _lib.ptr(m_rows), m, code, ws.data_ptr(), nbytes)
     return ids, logp

@@ -394,7 +394,7 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
 
 /* Bytes of hk_sample's workspace (16-byte aligned) on `device`; cuts: whether
  * top-k or top-p may be on (a pointer given, 0 < top_k < cols or top_p < 1). */
-size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int device);
+size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int dtype, int device);
 
 /* Bytes of device workspace hk_grpo_loss_fwd needs. */
 size_t hk_grpo_workspace_size(int64_t B, int64_t L);

@@ -270,7 +270,7 @@ def test_workspace_is_checked():
     dev = gpu()
     x, u = torch.zeros(4, 5000, device=dev), torch.zeros(4, device=dev)
     ids, logp = torch.empty(4, dtype=torch.int64, device=dev), torch.empty(4, device=dev)
-    need = _lib.load().hk_sample_workspace_size(4, 5000, 1, dev.index)
+    need = _lib.load().hk_sample_workspace_size(4, 5000, 1, _lib.F32, dev.index)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     for nbytes, ok in ((need, True), (need - 256, False)):
         status = _lib.load().hk_sample(ids.data_ptr(), logp.data_ptr(), x.data_ptr(), u.data_ptr(), 4, 5000, 5000, None, 1.0,

@@ -198,7 +198,7 @@ def test_sample_refusals():
     _einval(call(ws=ctypes.c_void_p(264)), "aligned")
     assert call(rows=0) == 0
     # more for the cuts' bins, nothing that grows with rows * cols but the runs' records
-    small, large = (lib.hk_sample_workspace_size(256, 151936, cuts, 0) for cuts in (0, 1))
+    small, large = (lib.hk_sample_workspace_size(256, 151936, cuts, 2, 0) for cuts in (0, 1))
     assert 0 < small < large < 64 * 2 ** 20
-    assert lib.hk_sample_workspace_size(1 << 20, 300, 1, 0) < 64 * 2 ** 20
-    assert lib.hk_sample_workspace_size(-1, 300, 1, 0) == lib.hk_sample_workspace_size(4, 0, 1, 0) == 0
+    assert lib.hk_sample_workspace_size(1 << 20, 300, 1, 2, 0) < 64 * 2 ** 20
+    assert lib.hk_sample_workspace_size(-1, 300, 1, 2, 0) == lib.hk_sample_workspace_size(4, 0, 1, 2, 0) == 0
