@@ -13,18 +13,18 @@
 //
 // Nothing is sorted. The kept set is a threshold x* and a number of ties at
 // x* that are kept (the first ones by index), found by selection. A row is cut
-// into runs of 2048 columns, its runs are dealt to the waves of a few blocks,
-// and up to five launches follow each other (the later ones read the row from
-// the Infinity Cache):
-//   scan  max and log-sum-exp (fp32); for a row without filters the fp64 mass
-//         of each run instead
+// into runs of 512 to 2048 columns, its runs are dealt to the waves of a few
+// blocks, and up to five launches follow each other (the later ones read the
+// row from the Infinity Cache):
+//   scan  max and log-sum-exp (fp32); in a call without filters (open) the
+//         fp64 mass of each run instead
 //   hist  counts, and for top-p masses, in kBins bins linear in max - x
 //   cut   the bins of a row's blocks together; the bin that holds the cut; if
 //         several values may lie in it, the same over ranges of ordered keys,
 //         11 bits at a time, until one is left: x* and how many ties are kept
 //   mass  the kept mass of each run
 //   pick  the run that u * total falls into, and the token inside it
-// A call whose settings are numbers launches those it needs: scan and pick
+// A call whose settings are numbers launches those it needs: open and pick
 // without filters, scan, mass and pick with min-p alone.
 //
 // Masses are fp64: with 32-bit ones the running sums of a flat row of 1e5
@@ -47,7 +47,6 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kRun = 2048;            // columns of a run: 32 a lane
 constexpr int kLanes = 1024;          // threads of a block
 constexpr int kWaves = kLanes / kWave;
 constexpr int kMaxSplit = 16;         // blocks a row
@@ -56,7 +55,7 @@ constexpr int kFineBins = 2048;
 constexpr double kRange = 24;
 constexpr double kTempMin = 0x1p-64, kTempMax = 0x1p64;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
-constexpr int kMaxQuarters = 1024;    // quarter maxima that a bound on the k-th logit is taken from
+constexpr int kGroups = 256;          // maxima that a bound on the k-th logit is taken from
 
 // A setting of every row, or one each.
 struct Setting {
@@ -107,6 +106,7 @@ template <typename T> struct Hist {
 struct Cut {
   float x;
   uint32_t ties, equal;
+  uint32_t count;  // logits kept
 };
 struct SampleArgs {
   int64_t* ids;
@@ -118,16 +118,17 @@ struct SampleArgs {
   int top_k_wide;
   int64_t top_k;
   int64_t ld;
-  int cols, runs;  // runs of a row
+  int cols, run_cols, runs;  // columns of a run (512, 1024 or 2048), runs of a row
   int split;       // blocks of a row
+  int open;        // no row has a filter
   int has_cuts;    // cuts is written
   double magic;    // 2^(52 - b): e + magic holds e in b fixed-point bits
   // workspace
   float *part_max, *part_sum;  // [rows][split]
-  float* quarters;             // [rows][4 runs] maxima of 512 columns
+  float* quarters;             // [rows][4 runs] maxima of a quarter of a run's columns (those of 16 lanes)
   double* run_mass;            // [rows][runs]
   uint32_t* run_ties;
-  float *run_max, *run_ref;    // of open rows: the run's maximum, and the logit whose mass its masses take as 1
+  float *run_max, *run_ref;    // of an open call: the run's maximum, and the logit whose mass its masses take as 1
   void* hist;                  // Hist<T> [rows][split], split > 1
   Cut* cuts;                   // [rows]
 };
@@ -139,7 +140,7 @@ struct Asked {
   double temp, top_p, min_p;
   double k;  // log2(e) / T
   int64_t top_k;
-  bool by_k, by_p, open;  // open: no filter at all
+  bool by_k, by_p;
   bool in_range;
 };
 __device__ __forceinline__ Asked asked(const SampleArgs& g, int64_t row) {
@@ -155,7 +156,6 @@ __device__ __forceinline__ Asked asked(const SampleArgs& g, int64_t row) {
   a.k = kLog2eD / a.temp;
   a.by_k = a.top_k > 0 && a.top_k < g.cols;
   a.by_p = a.top_p < 1.0;
-  a.open = !a.by_k && !a.by_p && !(a.min_p > 0.0);
   a.in_range = a.temp >= kTempMin && a.temp <= kTempMax && u >= 0.f && u <= 1.f && a.top_p == a.top_p &&
                a.min_p == a.min_p;
   return a;
@@ -210,32 +210,48 @@ __device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_cols(const T* row, int c
   if (c + VEC <= cols) return load_pack_any<T, VEC>(row + c);
   float f[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) f[i] = c + i < cols ? to_f32<T>(row[c + i]) : -INFINITY;
+  for (int i = 0; i < VEC; ++i) f[i] = -INFINITY;
+  if (c < cols) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (c + i < cols) f[i] = to_f32<T>(row[c + i]);
+  }
   return pack<T, VEC>(f);
 }
 
-// A row's runs first, first + waves, ...: look(pack, column) for each 16 bytes of a lane, done(run) after each run. A
-// wave has two packs on their way. The loop stays rolled: unrolled over a run (32 logits a lane) these kernels have 25
-// to 80 KB of code, and fetching it, not the logits, set their time (hist of 64 x 151936: 33 us; 11 rolled).
+// A row's runs first, first + waves, ...: look(pack) for each 16 bytes of a lane, done(run) after each run. A wave has
+// two packs on their way. The loop stays rolled: unrolled over a run (32 logits a lane) these kernels have 25 to 80 KB
+// of code, and fetching it, not the logits, set their time (hist of 64 x 151936: 33 us; 24 rolled).
 template <typename T, typename L, typename D>
-__device__ __forceinline__ void each_run(const T* row, int cols, int runs, int first, int waves, L&& look, D&& done) {
-  constexpr int VEC = 16 / sizeof(T), kStep = kWave * VEC, kPacks = kRun / kStep;
+__device__ __forceinline__ void each_run(const T* row, int cols, int run_cols, int runs, int first, int waves, L&& look,
+                                         D&& done) {
+  constexpr int VEC = 16 / sizeof(T), kStep = kWave * VEC;
+  first = __builtin_amdgcn_readfirstlane(first);  // (the wave's: the loop runs on the scalar unit)
   if (first >= runs) return;
   const int lane_col = (int)(threadIdx.x % kWave) * VEC;
-  int ahead = first, ahead_pack = 2;
-  Pack<T, VEC> p0 = load_cols(row, first * kRun + lane_col, cols);
-  Pack<T, VEC> p1 = load_cols(row, first * kRun + kStep + lane_col, cols);
-  for (int run = first; run < runs; run += waves) {
+  int run = first, at = 0, ahead = first, ahead_at = 0;
+  auto load = [&] {
+    const int c = ahead * run_cols + ahead_at;
+    Pack<T, VEC> p;
+    if (ahead < runs && c + kStep <= cols) p = load_pack_any<T, VEC>(row + c + lane_col);
+    else p = load_cols(row, c + lane_col, ahead < runs ? cols : 0);
+    ahead_at += kStep;
+    if (ahead_at == run_cols) ahead_at = 0, ahead += waves;
+    return p;
+  };
+  Pack<T, VEC> p0 = load(), p1 = load();
 #pragma unroll 1
-    for (int j = 0; j < kPacks; ++j) {
-      const Pack<T, VEC> p = p0;
-      p0 = p1;
-      if (ahead_pack == kPacks) ahead_pack = 0, ahead += waves;
-      if (ahead < runs) p1 = load_cols(row, ahead * kRun + ahead_pack * kStep + lane_col, cols);
-      ++ahead_pack;
-      look(p, run * kRun + j * kStep + lane_col);
+  while (run < runs) {
+    const Pack<T, VEC> p = p0;
+    p0 = p1;
+    p1 = load();
+    look(p);
+    at += kStep;
+    if (at == run_cols) {
+      done(run);
+      at = 0;
+      run += waves;
     }
-    done(run);
   }
 }
 
@@ -279,23 +295,27 @@ template <typename X> __device__ __forceinline__ X wave_total(X v) {
   v += moved<dpp::kBcast31, 0xc>(v);
   return of_lane63(v);
 }
-// sum over the threads before this one; `tmp` holds one value a wave and, after it, their totals
-template <typename X> __device__ __forceinline__ X block_before(X v, X* tmp) {
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+template <typename X> __device__ __forceinline__ X of_lane(X v, int lane) {
+  if constexpr (sizeof(X) == 4) {
+    return __builtin_bit_cast(X, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const u32x2 w = __builtin_bit_cast(u32x2, v);
+    return __builtin_bit_cast(X, u32x2{(uint32_t)__builtin_amdgcn_readlane((int)w.x, lane),
+                                       (uint32_t)__builtin_amdgcn_readlane((int)w.y, lane)});
+  }
+}
+// the sum over the threads before this one, and over all; `tmp` holds one value a wave
+template <typename X> __device__ __forceinline__ X block_before(X v, X* tmp, X* total) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
   const X incl = wave_scan(v);
   __syncthreads();
   if (lane == kWave - 1) tmp[wave] = incl;
   __syncthreads();
+  const X waves = wave_scan(lane < kWaves ? tmp[lane] : X(0));
+  *total = of_lane63(waves);
   X before = incl - v;
-#pragma unroll 1
-  for (int i = 0; i < wave; ++i) before += tmp[i];
+  if (wave > 0) before += of_lane(waves, wave - 1);
   return before;
-}
-template <typename X> __device__ __forceinline__ X total_of(const X* tmp) {
-  X t = tmp[0];
-#pragma unroll 1
-  for (int i = 1; i < kWaves; ++i) t += tmp[i];
-  return t;
 }
 
 // The first thread of the block for which `passes`, or if there is none the last for which `some`; -1 without either.
@@ -326,10 +346,10 @@ struct Start {
     const int lane = threadIdx.x % kWave;
     const float m = lane < g.split ? g.part_max[row * g.split + lane] : -INFINITY;
     const float s = lane < g.split ? g.part_sum[row * g.split + lane] : 0.f;
-    cut = {-INFINITY, 0xffffffffu, 0};
+    cut = {-INFINITY, 0xffffffffu, 0, 0xffffffffu};
     if (with_cut && g.has_cuts) cut = g.cuts[row];
     a = asked(g, row);
-    if (!a.by_k && !a.by_p) cut = {-INFINITY, 0xffffffffu, 0};
+    if (!a.by_k && !a.by_p) cut = {-INFINITY, 0xffffffffu, 0, 0xffffffffu};
     max = wave_max(m);
     sum = wave_sum(m == -INFINITY ? s : s * exp2_fast((m - max) * (float)a.k));
     // (a NaN, a +inf or nothing above -inf leaves the sum NaN or 0)
@@ -342,10 +362,25 @@ struct Start {
       const double least = (double)max + a.temp * kLn2D * (y + kLog2eD * (rest - 0.5 * rest * rest));
       float f = (float)(p < 1.0 ? least : (double)max);
       if (p < 1.0 && (double)f < least) f = nextafterf(f, INFINITY);
-      if (f > cut.x) cut = {f, 0xffffffffu, 0};
+      if (f > cut.x) cut = {f, 0xffffffffu, 0, cut.count};
     }
   }
 };
+
+// f(logit) for those of a pack that are in a bin of several values and above -inf. Few are, so the loop stays rolled: the
+// pack moves down by one logit a turn.
+template <typename F>
+__device__ __forceinline__ void each_several(Pack<__bf16, 8> p, F&& f) {
+  typedef Bins<__bf16> B;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const float v = bits_f32(p.w[0] << 16);
+    if (B::several(B::of(v)) && v != -INFINITY) f(v);
+#pragma unroll
+    for (int j = 0; j < 3; ++j) p.w[j] = __builtin_amdgcn_alignbit(p.w[j + 1], p.w[j], 16);
+    p.w[3] >>= 16;
+  }
+}
 
 // bf16: the masses of the bins that hold one value, 0 in the others, whose logits are looked at one by one.
 template <typename F>
@@ -355,11 +390,10 @@ __device__ __forceinline__ void fill_table(double* table, F&& mass) {
   for (int b = threadIdx.x; b < B::kUsed; b += kLanes) table[b] = B::several(b) ? 0.0 : mass(B::value(b));
   __syncthreads();
 }
-// The sum of the table's masses over a pack, and of `mass` over its logits of the other bins (from column c of the row;
-// those are few). *least: the lowest bin met so far, *most the highest rank.
+// The sum of the table's masses over a pack, and of `mass` over its few logits of the other bins; 0 if no logit of the
+// wave comes up to the bin `reach`.
 template <typename F>
-__device__ __forceinline__ double sum_table(const double* table, const Pack<__bf16, 8>& p, const __bf16* row, int c, int cols,
-                                            int reach, F&& mass) {
+__device__ __forceinline__ double sum_table(const double* table, const Pack<__bf16, 8>& p, int reach, F&& mass) {
   typedef Bins<__bf16> B;
   B::Two bins[4], least = (B::Two)((short)B::kUsed), low = (B::Two)((short)B::kSide), high = (B::Two)((short)0);
 #pragma unroll
@@ -374,13 +408,7 @@ __device__ __forceinline__ double sum_table(const double* table, const Pack<__bf
   if (__any(min(least.x, least.y) <= reach)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) s0 += table[bins[j].x], s1 += table[bins[j].y];
-    if (min(low.x, low.y) == 0 || max(high.x, high.y) > B::kSide) {
-#pragma unroll 1
-      for (int i = c; i < min(c + 8, cols); ++i) {
-        const float v = to_f32<__bf16>(row[i]);
-        if (B::several(B::of(v)) && v != -INFINITY) s0 += mass(v);
-      }
-    }
+    if (min(low.x, low.y) == 0 || max(high.x, high.y) > B::kSide) each_several(p, [&](float v) { s0 += mass(v); });
   }
   return s0 + s1;
 }
@@ -389,87 +417,20 @@ __device__ __forceinline__ double sum_table(const double* table, const Pack<__bf
 template <typename T>
 __global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
   constexpr int VEC = 16 / sizeof(T);
-  // an open row's masses of bf16 logits below 2^8 in size: 2^(x k) itself from the table, within 2^+-739
-  constexpr bool kTable = Bins<T>::kExact;
-  __shared__ double table[kTable ? Bins<__bf16>::kUsed : 1];
   __shared__ float sm[kWaves], sz[kWaves];
   const int64_t row = blockIdx.x / g.split;
   const int part = blockIdx.x % g.split;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const Asked a = asked(g, row);
   const T* x = static_cast<const T*>(g.logits) + row * g.ld;
-  const int first = part * kWaves + wave, waves = g.split * kWaves;
-  if (a.open) {
-    const bool use_table = kTable && a.temp >= 0.5;
-    if constexpr (kTable) {
-      if (use_table) fill_table(table, [&](float v) { return exp2_product((double)v, a.k); });
-    }
-    // m: this lane's maximum in the run, and (without the table) the logit whose mass is 1
-    float m = -INFINITY;
-    double mass = 0.0;
-    auto by_polynomial = [&](const Pack<T, VEC>& p, int) {
-      float v[VEC], n = m;
-      unpack(p, v);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) n = fmaxf(n, v[i]);
-      const double ref = n == -INFINITY ? 0.0 : (double)n;
-      if (__any(n > m) && mass > 0.0) mass *= exp2_product((double)m - ref, a.k);
-      m = n;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) mass += exp2_product((double)v[i] - ref, a.k);
-    };
-    auto finish = [&](int run, bool table_done) {
-      const float rm = wave_max(m);
-      float ref = rm == -INFINITY ? 0.f : rm;
-      if (table_done) ref = 0.f;
-      else if (m != -INFINITY) mass *= exp2_product((double)m - (double)ref, a.k);
-      mass = wave_total(mass);
-      if (lane == 0) {
-        g.run_mass[row * g.runs + run] = mass;
-        g.run_max[row * g.runs + run] = rm;
-        g.run_ref[row * g.runs + run] = ref;
-      }
-      m = -INFINITY;
-      mass = 0.0;
-    };
-    if constexpr (kTable) {
-      if (use_table) {
-        each_run(
-            x, g.cols, g.runs, first, waves,
-            [&](const Pack<T, VEC>& p, int c) {
-              float v[VEC];
-              unpack(p, v);
-#pragma unroll
-              for (int i = 0; i < VEC; ++i) m = fmaxf(m, v[i]);
-              // (a logit of 2^8 or more in size may take this sum out of range; the run is then done again)
-              mass += sum_table(table, p, x, c, g.cols, Bins<T>::kUsed,
-                                [&](float y) { return exp2_product((double)y, a.k); });
-            },
-            [&](int run) {
-              const float rm = wave_max(m);
-              if (fabsf(rm) >= 0x1p8f) {
-                m = -INFINITY;
-                mass = 0.0;
-                each_run(x, g.cols, run + 1, run, 1, by_polynomial, [](int) {});
-                finish(run, false);
-              } else {
-                finish(run, true);
-              }
-            });
-        return;
-      }
-    }
-    each_run(x, g.cols, g.runs, first, waves, by_polynomial, [&](int run) { finish(run, false); });
-    return;
-  }
   const float c = (float)a.k;
   float m = -INFINITY, z = 0.f, rm = -INFINITY;  // rm: of the run
   each_run(
-      x, g.cols, g.runs, first, waves,
-      [&](const Pack<T, VEC>& p, int) {
-        float v[VEC], q = v[0];
+      x, g.cols, g.run_cols, g.runs, part * kWaves + wave, g.split * kWaves,
+      [&](const Pack<T, VEC>& p) {
+        float v[VEC];
         unpack(p, v);
-        q = v[0];
+        float q = v[0];
 #pragma unroll
         for (int i = 1; i < VEC; ++i) q = fmaxf(q, v[i]);
         rm = fmaxf(rm, q);
@@ -504,6 +465,79 @@ __global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
   if (lane == 0) g.part_max[blockIdx.x] = bm, g.part_sum[blockIdx.x] = z;
 }
 
+// A call without filters: the mass of each run, and its maximum.
+template <typename T>
+__global__ __launch_bounds__(kLanes) void sample_open_kernel(SampleArgs g) {
+  constexpr int VEC = 16 / sizeof(T);
+  // masses of bf16 logits below 2^8 in size: 2^(x k) itself from the table, within 2^+-739. Worth its making for two
+  // runs a wave.
+  constexpr bool kTable = Bins<T>::kExact;
+  __shared__ double table[kTable ? Bins<__bf16>::kUsed : 1];
+  const int64_t row = blockIdx.x / g.split;
+  const int part = blockIdx.x % g.split;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const Asked a = asked(g, row);
+  const T* x = static_cast<const T*>(g.logits) + row * g.ld;
+  const int first = part * kWaves + wave, waves = g.split * kWaves;
+  const bool use_table = kTable && a.temp >= 0.5 && g.runs * (g.run_cols / 512) > 8 * waves;
+  if constexpr (kTable) {
+    if (use_table) fill_table(table, [&](float v) { return exp2_product((double)v, a.k); });
+  }
+  // m: this lane's maximum in the run, and (without the table) the logit whose mass is 1
+  float m = -INFINITY;
+  double mass = 0.0;
+  auto by_polynomial = [&](const Pack<T, VEC>& p) {
+    float v[VEC], n = m;
+    unpack(p, v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) n = fmaxf(n, v[i]);
+    const double ref = n == -INFINITY ? 0.0 : (double)n;
+    if (__any(n > m) && mass > 0.0) mass *= exp2_product((double)m - ref, a.k);
+    m = n;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) mass += exp2_product((double)v[i] - ref, a.k);
+  };
+  auto finish = [&](int run, bool table_done) {
+    const float rm = wave_max(m);
+    float ref = rm == -INFINITY ? 0.f : rm;
+    if (table_done) ref = 0.f;
+    else if (m != -INFINITY) mass *= exp2_product((double)m - (double)ref, a.k);
+    mass = wave_total(mass);
+    if (lane == 0) {
+      g.run_mass[row * g.runs + run] = mass;
+      g.run_max[row * g.runs + run] = rm;
+      g.run_ref[row * g.runs + run] = ref;
+    }
+    m = -INFINITY;
+    mass = 0.0;
+  };
+  if constexpr (kTable) {
+    if (use_table) {
+      each_run(
+          x, g.cols, g.run_cols, g.runs, first, waves,
+          [&](const Pack<T, VEC>& p) {
+            float v[VEC];
+            unpack(p, v);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) m = fmaxf(m, v[i]);
+            // (a logit of 2^8 or more in size may take this sum out of range; the run is then done again)
+            mass += sum_table(table, p, Bins<T>::kUsed, [&](float y) { return exp2_product((double)y, a.k); });
+          },
+          [&](int run) {
+            const bool again = fabsf(wave_max(m)) >= 0x1p8f;
+            if (again) {
+              m = -INFINITY;
+              mass = 0.0;
+              each_run(x, g.cols, g.run_cols, run + 1, run, 1, by_polynomial, [](int) {});
+            }
+            finish(run, !again);
+          });
+      return;
+    }
+  }
+  each_run(x, g.cols, g.run_cols, g.runs, first, waves, by_polynomial, [&](int run) { finish(run, false); });
+}
+
 // ---- hist and cut -----------------------------------------------------------
 struct Fine {
   u64 mass[kFineBins];
@@ -512,7 +546,8 @@ struct Fine {
 // What the bins of a block's columns need, and what finding a cut needs beside.
 template <typename T> struct HistShared {
   Hist<T> hist;
-  float least;
+  float groups[kGroups], best[kGroups / kWave];
+  int reach[kLanes];
 };
 template <typename T> struct CutShared : HistShared<T> {
   Fine fine;
@@ -530,7 +565,7 @@ struct Share {
   static constexpr int kEach = BINS / kLanes;
   static_assert(BINS % kLanes == 0, "whole turns");
   uint32_t count[kEach], total, before;
-  u64 mass[kEach], mass_total, mass_before;
+  u64 mass[kEach], mass_total, mass_before, all_mass;
   // (begins with a barrier)
   template <typename S, typename M>
   __device__ __forceinline__ Share(const uint32_t* counts, M&& mass_of, S& sh) : total(0), mass_total(0) {
@@ -540,8 +575,9 @@ struct Share {
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
       mass[i] = count[i] ? mass_of(kEach * (int)threadIdx.x + i, count[i]) : 0, mass_total += mass[i];
-    before = block_before<uint32_t>(total, sh.utmp);
-    mass_before = block_before<u64>(mass_total, sh.ltmp);
+    uint32_t all;
+    before = block_before<uint32_t>(total, sh.utmp, &all);
+    mass_before = block_before<u64>(mass_total, sh.ltmp, &all_mass);
   }
   // The bin whose running count reaches `count_target` (by count), or whose running mass reaches `mass_target`; what
   // lies before it goes to sh. Exactly one bin qualifies. Begins and ends with a barrier.
@@ -568,7 +604,7 @@ struct Row {
   static constexpr int VEC = 16 / sizeof(T);
   typedef Bins<T> B;
   const T* x;
-  int cols, runs;
+  int cols, run_cols, runs;
   float max;        // of the row
   double k;         // log2(e) / T
   float bin_step;   // linear bins: bins / (kRange T)
@@ -577,6 +613,7 @@ struct Row {
   __device__ __forceinline__ Row(const SampleArgs& g, int64_t row, const Start& st)
       : x(static_cast<const T*>(g.logits) + row * g.ld),
         cols(g.cols),
+        run_cols(g.run_cols),
         runs(g.runs),
         max(st.max),
         k(st.a.k),
@@ -616,8 +653,8 @@ struct Row {
       // (what is left out counts as low: the k-th logit lies above)
       const int reach = least == -INFINITY ? kLow - 1 : ::min(kLow - 1, B::of(least));
       each_run(
-          x, cols, runs, first, waves,
-          [&](const Pack<T, VEC>& p, int c) {
+          x, cols, run_cols, runs, first, waves,
+          [&](const Pack<T, VEC>& p) {
             typename B::Two low2 = (typename B::Two)((short)B::kSide), high2 = (typename B::Two)((short)0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -630,14 +667,8 @@ struct Row {
               if (b.y <= reach) atomicAdd(&h.count[b.y], 1u);
               else ++low;
             }
-            if (masses && (::min(low2.x, low2.y) == 0 || ::max(high2.x, high2.y) > B::kSide)) {
-#pragma unroll 1
-              for (int i = c; i < ::min(c + VEC, cols); ++i) {
-                const float v = to_f32<T>(x[i]);
-                const int b = B::of(v);
-                if (B::several(b) && v != -INFINITY) atomicAdd(&h.mass[B::slot(b)], fixed(mass(v)));
-              }
-            }
+            if (masses && (::min(low2.x, low2.y) == 0 || ::max(high2.x, high2.y) > B::kSide))
+              each_several(p, [&](float v) { atomicAdd(&h.mass[B::slot(B::of(v))], fixed(mass(v))); });
           },
           [](int) {});
       low = wave_total(low);
@@ -645,8 +676,8 @@ struct Row {
     } else {
       constexpr int kLow = B::kCount - 1;
       each_run(
-          x, cols, runs, first, waves,
-          [&](const Pack<T, VEC>& p, int) {
+          x, cols, run_cols, runs, first, waves,
+          [&](const Pack<T, VEC>& p) {
             float v[VEC];
             unpack(p, v);
             float most = v[0];
@@ -786,6 +817,7 @@ struct Row {
     const u64 each = masses ? fixed(mass(value)) : 0;
     // (by mass: the bin holds equal * each >= tau - above > 0)
     cut.ties = by_count ? count - cnt : (uint32_t)((tau - above + each - 1) / each);
+    cut.count = cnt + cut.ties;
     *kept = above + each * cut.ties;
     return cut;
   }
@@ -794,8 +826,8 @@ struct Row {
   __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a) const {
     const Share<B::kCount> share(
         sh.hist.count, [&](int b, uint32_t c) { return a.by_p ? mass_of_bin(sh.hist, b, c) : 0; }, sh);
-    u64 total = total_of(sh.ltmp);
-    Cut cut = {INFINITY, 0, 0};
+    u64 total = share.all_mass;
+    Cut cut = {INFINITY, 0, 0, 0};
     // by count, then by mass of what that kept
 #pragma unroll 1
     for (int turn = a.by_k ? 0 : 1; turn < (a.by_p ? 2 : 1); ++turn) {
@@ -803,62 +835,66 @@ struct Row {
       u64 kept;
       const Cut c = find_cut(sh, share, turn == 0, (uint32_t)a.top_k, tau, a.by_p, &kept);
       if (turn == 0 || !a.by_k || c.x > cut.x) cut = c;
-      else if (c.x == cut.x && c.ties < cut.ties) cut.ties = c.ties;
+      else if (c.x == cut.x && c.ties < cut.ties) cut.ties = c.ties, cut.count = c.count;
       total = kept;
     }
     return cut;
   }
 };
 
-// A lower bound of the k-th largest logit: the k-th largest of the maxima of 512 columns (each of those k is a logit of
-// its own) to 16 bits of key, where there are enough of them. The first wave finds it, bit by bit.
-__device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row, const Asked& a, float* shared) {
-  constexpr int kMost = kMaxQuarters / kWave;
-  const int n = 4 * g.runs;
-  if (!a.by_k || a.top_k > n || n > kMaxQuarters) return -INFINITY;
-  if (threadIdx.x < kWave) {
-    uint32_t key[kMost];
-#pragma unroll
-    for (int j = 0; j < kMost; ++j) {
-      const int i = j * kWave + (int)threadIdx.x;
-      key[j] = i < n ? key_of<__bf16>(g.quarters[row * n + i]) : 0;
-    }
-    uint32_t least = 0;
+// A lower bound of the k-th largest logit, k <= kGroups: the k-th largest of the maxima of kGroups disjoint sets of
+// columns (each of those k is a logit of its own), put together from the scan's. Its value is the largest that k of them
+// reach; four threads count for each.
+template <typename S>
+__device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row, const Asked& a, S& sh) {
+  static_assert(kLanes == 4 * kGroups, "four threads a group");
+  const int n = 4 * g.runs, i = threadIdx.x % kGroups, part = threadIdx.x / kGroups;
+  if (!a.by_k || a.top_k > min(n, kGroups)) return -INFINITY;
+  if (part == 0) {
+    float m = -INFINITY;
 #pragma unroll 1
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t tried = least | 1u << bit;
-      int count = 0;
-#pragma unroll
-      for (int j = 0; j < kMost; ++j)
-        if (j * kWave < n) count += __popcll(__ballot(key[j] >= tried));
-      if (count >= (int)a.top_k) least = tried;
-    }
-    // (0x7f: -inf)
-    if (threadIdx.x == 0)
-      *shared = least <= 0x7f ? -INFINITY : bits_f32((least & 0x8000u) ? (least ^ 0x8000u) << 16 : ~(least << 16));
+    for (int j = i; j < n; j += kGroups) m = fmaxf(m, g.quarters[row * n + j]);
+    sh.groups[i] = m;
   }
   __syncthreads();
-  return *shared;
+  const float m = sh.groups[i];
+  int reach = 0;
+#pragma unroll 4
+  for (int j = 0; j < kGroups / 4; ++j) reach += sh.groups[part * (kGroups / 4) + j] >= m ? 1 : 0;
+  sh.reach[threadIdx.x] = reach;
+  __syncthreads();
+  if (part == 0) {
+    for (int q = 1; q < 4; ++q) reach += sh.reach[q * kGroups + i];
+    const float best = wave_max(reach >= (int)a.top_k ? m : -INFINITY);
+    if (threadIdx.x % kWave == 0) sh.best[threadIdx.x / kWave] = best;
+  }
+  __syncthreads();
+  float best = sh.best[0];
+#pragma unroll
+  for (int w = 1; w < kGroups / kWave; ++w) best = fmaxf(best, sh.best[w]);
+  return best;
 }
 
 // WHOLE: one block has the whole row (split 1) and goes on to the cut.
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
-  __shared__ typename std::conditional<WHOLE, CutShared<T>, HistShared<T>>::type sh;
+  __shared__ __align__(16) typename std::conditional<WHOLE, CutShared<T>, HistShared<T>>::type sh;
   const int64_t row = blockIdx.x / g.split;
   const Start st(g, row, false);
   if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
   const Row<T> r(g, row, st);
-  r.fill(sh.hist, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, st.a, &sh.least), st.a.by_p);
+  r.fill(sh.hist, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, st.a, sh), st.a.by_p);
   if constexpr (WHOLE) {
     const Cut cut = r.find(sh, st.a);
     if (threadIdx.x == 0) g.cuts[row] = cut;
   } else {
     __syncthreads();
     Hist<T>& to = static_cast<Hist<T>*>(g.hist)[blockIdx.x];
-    for (int i = threadIdx.x; i < Bins<T>::kCount; i += kLanes) to.count[i] = sh.hist.count[i];
-    if (st.a.by_p)
-      for (int i = threadIdx.x; i < Bins<T>::kMasses; i += kLanes) to.mass[i] = sh.hist.mass[i];
+    static_assert(sizeof(Hist<T>) % 16 == 0 && Bins<T>::kMasses % 2 == 0, "whole vectors");
+    // (masses first; they are not read without top-p)
+    const int skip = st.a.by_p ? 0 : (int)(sizeof(u64) * Bins<T>::kMasses / 16);
+    for (int i = skip + (int)threadIdx.x; i < (int)(sizeof(Hist<T>) / 16); i += kLanes)
+      reinterpret_cast<u32x4*>(&to)[i] = reinterpret_cast<const u32x4*>(&sh.hist)[i];
   }
 }
 
@@ -907,52 +943,63 @@ __global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
   const int part = blockIdx.x % g.split;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const Start st(g, row, true);
-  if (!st.ok || st.a.open) return;
+  if (!st.ok) return;
   const Row<T> r(g, row, st);
   const Cut cut = st.cut;
   const bool all_ties = cut.ties >= cut.equal;
   auto kept = [&](float v) { return all_ties ? v >= cut.x : v > cut.x; };
-  int reach = 0;
-  if constexpr (kTable) {
-    fill_table(table, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
-    reach = Bins<T>::of(cut.x);
-  }
   double mass = 0.0;
-  uint32_t ties = 0;
+  uint32_t ties = 0;  // (the wave's)
+  const int first = part * kWaves + wave, waves = g.split * kWaves;
+  auto count_ties = [&](const Pack<T, VEC>& p) {
+    if (all_ties) return;
+    float v[VEC];
+    unpack(p, v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) ties += __popcll(__ballot(v[i] == cut.x));
+  };
+  auto done = [&](int run) {
+    mass = wave_total(mass);
+    if (lane == 0) g.run_mass[row * g.runs + run] = mass, g.run_ties[row * g.runs + run] = ties;
+    mass = 0.0;
+    ties = 0;
+  };
+  if constexpr (kTable) {
+    // few are kept: the table costs more than their polynomials (2 us; 1 in 64 of 38000 logits a block 0.6)
+    if (cut.count > (uint32_t)g.cols / 64) {
+      fill_table(table, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
+      const int reach = Bins<T>::of(cut.x);
+      each_run(
+          r.x, g.cols, g.run_cols, g.runs, first, waves,
+          [&](const Pack<T, VEC>& p) {
+            mass += sum_table(table, p, reach, [&](float y) { return kept(y) ? r.mass(y) : 0.0; });
+            count_ties(p);
+          },
+          done);
+      return;
+    }
+  }
   each_run(
-      r.x, g.cols, g.runs, part * kWaves + wave, g.split * kWaves,
-      [&](const Pack<T, VEC>& p, int c) {
+      r.x, g.cols, g.run_cols, g.runs, first, waves,
+      [&](const Pack<T, VEC>& p) {
         float v[VEC];
         unpack(p, v);
-        if constexpr (kTable) {
-          mass += sum_table(table, p, r.x, c, g.cols, reach, [&](float y) { return kept(y) ? r.mass(y) : 0.0; });
-        } else {
-          float most = v[0];
+        float most = v[0];
 #pragma unroll
-          for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
-          if (__any(most >= cut.x)) {
+        for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
+        if (__any(most >= cut.x)) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) mass += kept(v[i]) ? r.mass(v[i]) : 0.0;
-          }
-        }
-        if (!all_ties) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) ties += v[i] == cut.x ? 1 : 0;
+          for (int i = 0; i < VEC; ++i) mass += kept(v[i]) ? r.mass(v[i]) : 0.0;
+          count_ties(p);
         }
       },
-      [&](int run) {
-        mass = wave_total(mass);
-        ties = wave_total(ties);
-        if (lane == 0) g.run_mass[row * g.runs + run] = mass, g.run_ties[row * g.runs + run] = ties;
-        mass = 0.0;
-        ties = 0;
-      });
+      done);
 }
 
 // ---- pick -------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
-  constexpr int kCols = kRun / kLanes;  // columns a thread, in order
+  constexpr int kCols = 2;  // columns a thread, in order: runs of up to 2048
   __shared__ double dtmp[kWaves];
   __shared__ uint32_t utmp[kWaves];
   __shared__ float ftmp[kWaves];
@@ -976,7 +1023,7 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
   const float u = g.u[row];
 
   bool fine = a.in_range;
-  if (a.open) {
+  if (g.open) {
     float m = -INFINITY;
     for (int i = r0; i < r1; ++i) m = fmaxf(m, i == r0 ? max0 : run_max[i]);
     m = wave_max(m);
@@ -993,7 +1040,7 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
   }
   const float max = st.max;
   const Row<T> r(g, row, st);
-  const Cut cut = a.open ? Cut{-INFINITY, 0xffffffffu, 0} : st.cut;
+  const Cut cut = g.open ? Cut{-INFINITY, 0xffffffffu, 0, 0} : st.cut;
   const bool all_ties = cut.ties >= cut.equal;
   const double each = all_ties ? 0.0 : r.mass(cut.x);
 
@@ -1001,11 +1048,12 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
   uint32_t ties = 0, seen = 0;
   if (!all_ties) {
     for (int i = r0; i < r1; ++i) ties += i == r0 ? ties0 : run_ties[i];
-    seen = block_before<uint32_t>(ties, utmp);
+    uint32_t all;
+    seen = block_before<uint32_t>(ties, utmp, &all);
   }
   auto mass_of = [&](int i, uint32_t& ties_before) {
     const double m = i == r0 ? mass0 : run_mass[i];
-    if (a.open) return m * exp2_product((double)(i == r0 ? ref0 : run_ref[i]) - (double)max, r.k);
+    if (g.open) return m * exp2_product((double)(i == r0 ? ref0 : run_ref[i]) - (double)max, r.k);
     if (all_ties) return m;
     const uint32_t t = i == r0 ? ties0 : run_ties[i], left = cut.ties - min(cut.ties, ties_before);
     ties_before += t;
@@ -1015,8 +1063,8 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
   uint32_t rank = seen;
 #pragma unroll 1
   for (int i = r0; i < r1; ++i) mass += mass_of(i, rank);
-  const double before = block_before<double>(mass, dtmp);
-  const double total = total_of(dtmp);
+  double total;
+  const double before = block_before<double>(mass, dtmp, &total);
   if (!(total > 0.0 && total < INFINITY && max < INFINITY)) {  // (only an open row's can be)
     if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
     return;
@@ -1038,17 +1086,18 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
     sh_run = run;
   }
   __syncthreads();
-  const int c0 = sh_run * kRun + (int)threadIdx.x * kCols;
+  const int c0 = sh_run * g.run_cols + (int)threadIdx.x * kCols, c1 = min(g.cols, (sh_run + 1) * g.run_cols);
   float v[kCols];
 #pragma unroll
-  for (int i = 0; i < kCols; ++i) v[i] = c0 + i < g.cols ? to_f32<T>(r.x[c0 + i]) : -INFINITY;
+  for (int i = 0; i < kCols; ++i) v[i] = c0 + i < c1 ? to_f32<T>(r.x[c0 + i]) : -INFINITY;
   rank = sh_ties;
   const double base = sh_base;
   if (!all_ties) {
     ties = 0;
 #pragma unroll
     for (int i = 0; i < kCols; ++i) ties += v[i] == cut.x ? 1 : 0;
-    rank += block_before<uint32_t>(ties, utmp);
+    uint32_t all;
+    rank += block_before<uint32_t>(ties, utmp, &all);
   }
   double e[kCols];
   mass = 0.0;
@@ -1059,7 +1108,8 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
     e[i] = keep ? r.mass(v[i]) : 0.0;
     mass += e[i];
   }
-  double s = base + block_before<double>(mass, dtmp);
+  double run_total;
+  double s = base + block_before<double>(mass, dtmp, &run_total);
   if ((int)threadIdx.x != first_or_last(mass > 0.0 && s + mass > target, mass > 0.0, itmp)) return;
   int id = -1;
   float at = 0.f;
@@ -1071,19 +1121,31 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
     done = done || (e[i] > 0.0 && s > target);
   }
   g.ids[row] = id;
-  g.logp[row] = (float)(((double)at - (double)max) * r.k * kLn2D) - log_fast(a.open ? (float)total : st.sum);
+  g.logp[row] = (float)(((double)at - (double)max) * r.k * kLn2D) - log_fast(g.open ? (float)total : st.sum);
 }
 
-// Blocks a row: enough for two blocks a CU, each with a run a wave at least.
-int split_of(int64_t rows, int64_t runs, int64_t cus) {
-  const int64_t want = cdiv(2 * cus, std::max<int64_t>(rows, 1));
-  return (int)std::max<int64_t>(1, std::min<int64_t>({want, (int64_t)kMaxSplit, cdiv(runs, (int64_t)kWaves)}));
+// How a call is cut up. Two blocks a CU, so want = 2 CUs / rows blocks a row; runs as long as they can be (each costs a
+// sum over the wave) while there are four for every wave, so that no wave has much more than another; and of the blocks
+// that need the same number of turns, the fewest.
+struct Shape {
+  int64_t run_cols, runs, split;
+};
+Shape shape_of(int64_t rows, int64_t cols, int64_t cus) {
+  Shape s;
+  s.run_cols = 2048;
+  while (s.run_cols > 512 && rows * cdiv(cols, s.run_cols) < 8 * cus * kWaves) s.run_cols /= 2;
+  s.runs = cdiv(cols, s.run_cols);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 2 * cus / std::max<int64_t>(rows, 1)));
+  const int64_t turns = cdiv(s.runs, want * kWaves);
+  s.split = cdiv(s.runs, turns * kWaves);
+  return s;
 }
 
 struct Layout {
   size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, run_ref, hist, cuts, total;
 };
-Layout layout_of(int64_t rows, int64_t runs, int64_t split, bool cuts, bool bf16) {
+Layout layout_of(int64_t rows, const Shape& shape, bool cuts, bool bf16) {
+  const int64_t runs = shape.runs, split = shape.split;
   Layout l = {};
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -1116,8 +1178,7 @@ extern "C" {
 size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int dtype, int device) {
   if (rows < 0 || rows >= (1LL << 31) || cols <= 0 || cols > (1 << 30)) return 0;
   const int cus = cu_count(device);
-  const int64_t runs = cdiv(cols, (int64_t)kRun);
-  return std::max<size_t>(256, layout_of(rows, runs, split_of(rows, runs, cus > 0 ? cus : 256), cuts != 0, dtype == kBF16).total);
+  return std::max<size_t>(256, layout_of(rows, shape_of(rows, cols, cus > 0 ? cus : 256), cuts != 0, dtype == kBF16).total);
 }
 
 int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int64_t rows, int64_t cols, int64_t ld,
@@ -1141,12 +1202,12 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   const int dev = current_device();
   if (dev < 0) return (int)hipErrorNoDevice;
   const int cus = cu_count(dev);
-  const int64_t runs = cdiv(cols, (int64_t)kRun);
-  const int split = split_of(rows, runs, cus > 0 ? cus : 256);
+  const Shape shape = shape_of(rows, cols, cus > 0 ? cus : 256);
+  const int split = (int)shape.split;
   HK_REQUIRE(rows * split < (1LL << 31), "rows=%lld too large", (long long)rows);
   const bool cuts = top_k_rows || (top_k > 0 && top_k < cols) || top_p_rows || top_p < 1;
   const bool masses = cuts || min_p_rows || min_p > 0;
-  const Layout l = layout_of(rows, runs, split, cuts, dtype == kBF16);
+  const Layout l = layout_of(rows, shape, cuts, dtype == kBF16);
   HK_REQUIRE(workspace_bytes >= l.total, "workspace too small: need %zu bytes, got %zu", l.total, workspace_bytes);
   char* ws = (char*)workspace;
   SampleArgs g = {};
@@ -1162,11 +1223,13 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   g.top_k = top_k;
   g.ld = ld;
   g.cols = (int)cols;
-  g.runs = (int)runs;
+  g.run_cols = (int)shape.run_cols;
+  g.runs = (int)shape.runs;
   g.split = split;
+  g.open = !masses;
   g.has_cuts = cuts;
   int log2_cols = 0;
-  while ((1LL << log2_cols) < cols + kRun) ++log2_cols;
+  while ((1LL << log2_cols) < cols + 2048) ++log2_cols;  // (with the last run's filling)
   g.magic = (double)(1ULL << (52 - std::min(43, 63 - log2_cols)));
   g.part_max = (float*)(ws + l.part_max);
   g.part_sum = (float*)(ws + l.part_sum);
@@ -1181,7 +1244,8 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
     using T = decltype(tag);
     const hipStream_t st = (hipStream_t)stream;
     const dim3 parts((unsigned)(rows * split)), each((unsigned)rows);
-    hipLaunchKernelGGL((sample_scan_kernel<T>), parts, dim3(kLanes), 0, st, g);
+    if (masses) hipLaunchKernelGGL((sample_scan_kernel<T>), parts, dim3(kLanes), 0, st, g);
+    else hipLaunchKernelGGL((sample_open_kernel<T>), parts, dim3(kLanes), 0, st, g);
     if (const int rc = check_launch("sample_scan_kernel")) return rc;
     if (cuts) {
       if (split == 1) hipLaunchKernelGGL((sample_hist_kernel<T, true>), parts, dim3(kLanes), 0, st, g);

@@ -18,20 +18,21 @@ import torch
 from . import _lib
 
 
-def rms_norm_quant_forward(X, W, eps=1e-6, group_size=None, R=None):
-    """Forward. Returns (Q, scale, S, RSTD): Q float8_e4m3fn of X's shape, scale fp32 X.shape[:-1] + (groups,), S = X + R
-    (X itself without R), RSTD fp32 of the rows."""
+def _forward(X, W, eps, group_size, R, want_rstd):
+    # (host time: a decode step's call is bound by it, so only what is asked for is allocated)
+    dev = _lib.require_device(X, R, W)
     shape = X.shape
     hidden = shape[-1]
     assert W.dim() == 1 and W.shape[0] == hidden, f"Hidden dim mismatch: {hidden} vs {tuple(W.shape)}"
-    dev = _lib.require_device(X, R, W)
     if R is not None:
         assert R.shape == shape, f"X and R shapes differ: {tuple(shape)} vs {tuple(R.shape)}"
-    group = 0 if group_size is None else int(group_size)
-    if group_size is not None and group not in (32, 64, 128, 256):
-        raise ValueError(f"group_size must be None (the row), 32, 64, 128 or 256, got {group_size}")
-    if group and hidden % group:
-        raise ValueError(f"the hidden size {hidden} is not a multiple of group_size {group}")
+    group = 0
+    if group_size is not None:
+        group = int(group_size)
+        if group not in (32, 64, 128, 256):
+            raise ValueError(f"group_size must be None (the row), 32, 64, 128 or 256, got {group_size}")
+        if hidden % group:
+            raise ValueError(f"the hidden size {hidden} is not a multiple of group_size {group}")
     X = X.contiguous()
     W = W.contiguous()
     n_rows = X.numel() // hidden if hidden else 0
@@ -41,17 +42,24 @@ def rms_norm_quant_forward(X, W, eps=1e-6, group_size=None, R=None):
         if R.dtype != X.dtype:
             R = R.to(X.dtype)
         S = torch.empty_like(X)
-    Q = torch.empty(shape, dtype=torch.float8_e4m3fn, device=dev)
+    Q = torch.empty_like(X, dtype=torch.float8_e4m3fn)
     scale = torch.empty((*shape[:-1], hidden // group if group else 1), dtype=torch.float32, device=dev)
-    RSTD = torch.empty(n_rows, dtype=torch.float32, device=dev)
+    RSTD = torch.empty(n_rows, dtype=torch.float32, device=dev) if want_rstd else None
     _lib.call_on(dev, "hk_rms_norm_quant_fwd", Q.data_ptr(), scale.data_ptr(), None if R is None else S.data_ptr(),
-                 RSTD.data_ptr(), X.data_ptr(), _lib.ptr(R), W.data_ptr(), n_rows, hidden, hidden, group,
-                 _lib.dtype_code(X), _lib.dtype_code(W), float(eps))
+                 _lib.ptr(RSTD), X.data_ptr(), _lib.ptr(R), W.data_ptr(), n_rows, hidden, hidden, group,
+                 _lib.dtype_code(X), _lib.dtype_code(W), eps)
     return Q, scale, S, RSTD
 
 
+def rms_norm_quant_forward(X, W, eps=1e-6, group_size=None, R=None):
+    """Forward. Returns (Q, scale, S, RSTD): Q float8_e4m3fn of X's shape, scale fp32 X.shape[:-1] + (groups,), S = X + R
+    (X itself without R), RSTD fp32 of the rows."""
+    with torch.no_grad():
+        return _forward(X, W, eps, group_size, R, True)
+
+
 def _no_gradient(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if any(t.requires_grad for t in tensors):
         raise RuntimeError("the 8-bit norms have no gradient: call them under torch.no_grad(), or use "
                            "rms_norm_quant_forward with the unquantised norms' backward")
 
@@ -62,15 +70,17 @@ def hilda_rms_norm_quant(X, W, eps=1e-6, group_size=None):
     Q float8_e4m3fn; scale fp32 X.shape[:-1] + (1,), or + (H / group_size,) with group_size 32, 64, 128 or 256:
     max(max|Y| / 448, 2^-100) over the row or group.
     """
-    _no_gradient(X, W)
-    Q, scale, _, _ = rms_norm_quant_forward(X, W, eps, group_size)
+    if torch.is_grad_enabled():
+        _no_gradient(X, W)
+    Q, scale, _, _ = _forward(X, W, eps, group_size, None, False)
     return Q, scale
 
 
 def hilda_fused_add_rms_norm_quant(X, R, W, eps=1e-6, group_size=None):
     """S = X + R, Y = RMSNorm(S) * W in 8 bits: returns (Q, scale, S) with Y ~ Q * scale (see hilda_rms_norm_quant)."""
-    _no_gradient(X, R, W)
-    Q, scale, S, _ = rms_norm_quant_forward(X, W, eps, group_size, R)
+    if torch.is_grad_enabled():
+        _no_gradient(X, R, W)
+    Q, scale, S, _ = _forward(X, W, eps, group_size, R, False)
     return Q, scale, S
 
 

@@ -11,6 +11,7 @@ import torch
 
 from . import _lib
 
+_workspace_bytes: dict[tuple, int] = {}  # of a shape
 _TOP_K_CODE = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 
 
@@ -31,7 +32,6 @@ def _setting(value, shape, name, device):
     return _rows_of(value, shape, name, device), 0.0
 
 
-@torch.no_grad()
 def hilda_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draw a token for each row of logits (..., V): returns (ids, logp) of shape (...), int64 and fp32.
 
@@ -65,12 +65,17 @@ def hilda_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
         k = min(max(int(top_k), 0), vocab)
     strides = logits.stride()
     if len(strides) != 2 or strides[1] != 1 or strides[0] < vocab:
-        logits = logits.reshape(-1, vocab).contiguous()
+        logits = logits.detach().reshape(-1, vocab).contiguous()
     rows, code = logits.shape[0], _lib.dtype_code(logits)
     ids = torch.empty(shape, dtype=torch.int64, device=dev)
     logp = torch.empty(shape, dtype=torch.float32, device=dev)
     cuts = k_rows is not None or p_rows is not None or 0 < k < vocab or p < 1
-    nbytes = _lib.load().hk_sample_workspace_size(rows, vocab, cuts, code, dev.index)
+    key = (rows, vocab, cuts, code, dev.index)
+    nbytes = _workspace_bytes.get(key)
+    if nbytes is None:
+        nbytes = _lib.load().hk_sample_workspace_size(*key)
+        if len(_workspace_bytes) < 1024:
+            _workspace_bytes[key] = nbytes
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.call_on(dev, "hk_sample", ids.data_ptr(), logp.data_ptr(), logits.data_ptr(), uniform.data_ptr(), rows, vocab,
                  logits.stride(0) if rows > 1 else vocab, _lib.ptr(t_rows), t, _lib.ptr(k_rows), k_code, k,
