@@ -181,13 +181,13 @@ using namespace hk;
 
 extern "C" {
 
-int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int64_t q_in_sH, int64_t q_in_sT,
-                 int64_t q_out_sB, int64_t q_out_sH, int64_t q_out_sT, void* k_out, const void* k_in, int64_t Hk,
-                 int64_t k_in_sB, int64_t k_in_sH, int64_t k_in_sT, int64_t k_out_sB, int64_t k_out_sH,
-                 int64_t k_out_sT, const void* cos, const void* sin, int64_t table_rows, int64_t table_ld,
-                 const void* positions, int pos_type, int64_t pos_sA, int64_t pos_sB, int64_t pos_sT,
-                 const int64_t* sections, int axes, int interleaved, int64_t B, int64_t T, int64_t D, int dtype_x,
-                 int dtype_cs, int inverse, hk_stream_t stream) {
+int hk_rope_axes(void* q_out, const void* q_in, void* k_out, const void* k_in, const void* cos, const void* sin,
+                 const void* positions, const hk_rope_axes_shape* shape, hk_stream_t stream) {
+  HK_REQUIRE(shape != nullptr, "null pointer argument");
+  const int64_t B = shape->B, T = shape->T, D = shape->D, Hq = shape->Hq, Hk = shape->Hk;
+  const int64_t table_rows = shape->table_rows, table_ld = shape->table_ld;
+  const int64_t* sections = shape->sections;
+  const int axes = shape->axes, dtype_x = shape->dtype_x, dtype_cs = shape->dtype_cs, pos_type = shape->pos_type;
   HK_REQUIRE(B >= 0 && T >= 0 && Hq >= 0 && Hk >= 0 && D > 0, "invalid shape B=%lld T=%lld Hq=%lld Hk=%lld D=%lld",
              (long long)B, (long long)T, (long long)Hq, (long long)Hk, (long long)D);
   HK_REQUIRE(D % 2 == 0, "head_dim D=%lld must be even", (long long)D);
@@ -195,17 +195,16 @@ int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int
   HK_REQUIRE(dtype_x == kF32 || dtype_x == kF16 || dtype_x == kBF16, "invalid dtype code %d", dtype_x);
   HK_REQUIRE(pos_type == HK_I32 || pos_type == HK_I64, "positions must be int32 or int64, got code %d", pos_type);
   HK_REQUIRE(axes >= 1 && axes <= kMaxAxes, "1..%d position axes, got %d", kMaxAxes, axes);
-  HK_REQUIRE(sections != nullptr, "null pointer argument");
   const int64_t half = D / 2;
   RopeAxesArgs g = {};
   int64_t sum = 0;
   for (int a = 0; a < axes; ++a) {
     HK_REQUIRE(sections[a] >= 0, "sections must not be negative");
     sum += sections[a];
-    g.axes.n[a] = (int)(interleaved ? sections[a] : sum);
+    g.axes.n[a] = (int)(shape->interleaved ? sections[a] : sum);
   }
   HK_REQUIRE(sum == half, "sections sum to %lld, need D/2 = %lld", (long long)sum, (long long)half);
-  if (interleaved) {
+  if (shape->interleaved) {
     // axis a > 0 owns pairs a, a + A, ..., a + A (n_a - 1); all of them must exist
     for (int a = 1; a < axes; ++a)
       HK_REQUIRE(sections[a] == 0 || a + axes * (sections[a] - 1) < half,
@@ -213,10 +212,10 @@ int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int
                  (long long)half);
   }
   g.axes.count = axes;
-  g.axes.interleaved = interleaved ? 1 : 0;
-  const int64_t strides[] = {q_in_sB,  q_in_sH,  q_in_sT,  q_out_sB, q_out_sH, q_out_sT, k_in_sB, k_in_sH, k_in_sT,
-                             k_out_sB, k_out_sH, k_out_sT, pos_sA,   pos_sB,   pos_sT};
-  for (const int64_t s : strides) HK_REQUIRE(s >= 0, "negative strides are not supported");
+  g.axes.interleaved = shape->interleaved ? 1 : 0;
+  const int64_t* const strides[] = {shape->q_in, shape->q_out, shape->k_in, shape->k_out, shape->pos};
+  for (const int64_t* v : strides)
+    HK_REQUIRE(v[0] >= 0 && v[1] >= 0 && v[2] >= 0, "negative strides are not supported");
   HK_REQUIRE(table_rows >= 0 && table_ld >= half, "cos/sin row stride %lld smaller than D/2 = %lld",
              (long long)table_ld, (long long)half);
   HK_REQUIRE(B == 0 || T <= ((1LL << 31) - 1) / B, "B * T = %lld * %lld too large", (long long)B, (long long)T);
@@ -224,18 +223,21 @@ int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int
   if (B == 0 || T == 0 || Hq + Hk == 0) return HK_OK;
   HK_REQUIRE((Hq == 0 || (q_out && q_in)) && (Hk == 0 || (k_out && k_in)) && cos && sin && positions,
              "null pointer argument");
-  g.q = {(int)Hq, q_in_sB, q_in_sH, q_in_sT, q_out_sB, q_out_sH, q_out_sT};
-  g.k = {(int)Hk, k_in_sB, k_in_sH, k_in_sT, k_out_sB, k_out_sH, k_out_sT};
+  auto heads = [](int64_t n, const int64_t* in, const int64_t* out) {
+    return Heads{(int)n, in[0], in[1], in[2], out[0], out[1], out[2]};
+  };
+  g.q = heads(Hq, shape->q_in, shape->q_out);
+  g.k = heads(Hk, shape->k_in, shape->k_out);
   g.positions = positions;
-  g.ps_a = pos_sA;
-  g.ps_b = pos_sB;
-  g.ps_t = pos_sT;
+  g.ps_a = shape->pos[0];
+  g.ps_b = shape->pos[1];
+  g.ps_t = shape->pos[2];
   g.table_rows = table_rows;
   g.table_ld = table_ld;
   g.T = (uint32_t)T;
   g.half = (uint32_t)half;
   g.tokens = B * T;
-  g.sgn = inverse ? -1.f : 1.f;
+  g.sgn = shape->inverse ? -1.f : 1.f;
   // the storage order of the larger tensor decides how lanes walk memory
   const Heads& lead = Hq >= Hk ? g.q : g.k;
   const bool head_major = T > 1 && lead.is_t < lead.is_h;

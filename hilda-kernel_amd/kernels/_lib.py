@@ -43,8 +43,7 @@ SIGNATURES = {
     "hk_rope": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                        _i32, _i32, _i32, _p]),
     "hk_rope_qk": (_i32, [_p, _p] + [_i64] * 7 + [_p, _p] + [_i64] * 7 + [_p, _p] + [_i64] * 6 + [_i32, _i32, _i32, _p]),
-    "hk_rope_axes": (_i32, [_p, _p] + [_i64] * 7 + [_p, _p] + [_i64] * 7 + [_p, _p, _i64, _i64, _p, _i32, _i64, _i64, _i64,
-                            _p, _i32, _i32, _i64, _i64, _i64, _i32, _i32, _i32, _p]),
+    "hk_rope_axes": (_i32, [_p] * 9),
     "hk_rms_norm_quant_fwd": (_i32, [_p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i32, _i32, _f32, _p]),
     "hk_sample": (_i32, [_p, _p, _p, _p, _i64, _i64, _i64, _p, _f64, _p, _i32, _i64, _p, _f64, _p, _f64, _i32, _p, _sz,
                          _p]),
@@ -83,6 +82,17 @@ SIGNATURES = {
                                                _p, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32, _f32, _f32,
                                                _i32, _i64, _i64, _p, _sz, _p]),
 }
+
+
+
+class RopeAxesShape(ctypes.Structure):
+    """hk_rope_axes_shape"""
+
+    _fields_ = [(n, _i64) for n in ("B", "T", "D", "Hq", "Hk")] + \
+        [(n, _i64 * 3) for n in ("q_in", "q_out", "k_in", "k_out", "pos")] + \
+        [("table_rows", _i64), ("table_ld", _i64), ("sections", _i64 * 4)] + \
+        [(n, ctypes.c_int32) for n in ("axes", "interleaved", "pos_type", "dtype_x", "dtype_cs", "inverse")]
+
 
 ABI_VERSION = 2
 

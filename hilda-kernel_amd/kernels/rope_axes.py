@@ -18,65 +18,71 @@ from . import _lib
 from .rope import RotaryEmbedding
 
 _POS_CODE = {torch.int32: _lib.I32, torch.int64: _lib.I64}
-_sections_cache: dict[tuple, ctypes.Array] = {}
+# (device, hk_rope_axes_shape) of the layouts that have been checked, by everything the checks look at
+_shapes: dict[tuple, tuple] = {}
 
 
-def _sections_arg(sections):
-    """The sections as a C array (made once for each tuple of counts)."""
-    key = tuple(sections)
-    arr = _sections_cache.get(key)
-    if arr is None:
-        if not 1 <= len(key) <= 4:
-            raise ValueError(f"sections names 1 to 4 axes, got {len(key)}")
-        arr = (ctypes.c_int64 * len(key))(*(int(c) for c in key))
-        if len(_sections_cache) < 64:
-            _sections_cache[key] = arr
-    return arr
+def _row_stride(table):
+    """Elements from one row of a cos or sin table to the next (its width where there is no next)."""
+    return table.stride(-2) if table.shape[-2] > 1 else table.shape[-1]
+
+
+def _checked(q, k, cos, sin, positions, sections, interleaved, inverse):
+    """(device, shape) of a call whose head dims and table rows are contiguous; raises if it is not one."""
+    dev = _lib.require_device(q, k, cos, sin, positions)
+    assert q.dim() == 4 and k.dim() == 4, "q and k must be (bsz, n_heads, seq_len, head_dim)"
+    bsz, hq, seq_len, hd = q.shape
+    kb, hk, kt, kd = k.shape
+    assert (kb, kt, kd) == (bsz, seq_len, hd), f"q and k differ: {tuple(q.shape)} and {tuple(k.shape)}"
+    assert q.dtype == k.dtype, f"q and k have different dtypes: {q.dtype} and {k.dtype}"
+    assert cos.shape == sin.shape and cos.dtype == sin.dtype, "cos and sin must be alike"
+    assert (cos.dim() == 2 or cos.dim() == 3 and cos.shape[0] == 1) and cos.shape[-1] * 2 == hd, \
+        f"cos/sin must be (1, positions, head_dim/2); got {tuple(cos.shape)}"
+    axes = len(sections)
+    if not 1 <= axes <= 4:
+        raise ValueError(f"sections names 1 to 4 axes, got {axes}")
+    if positions.dtype not in _POS_CODE:
+        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+    assert positions.dim() == 3 and positions.shape[0] == axes and positions.shape[2] == seq_len and \
+        positions.shape[1] in (1, bsz), \
+        f"positions must be ({axes}, {bsz} or 1, {seq_len}); got {tuple(positions.shape)}"
+    s = _lib.RopeAxesShape(B=bsz, T=seq_len, D=hd, Hq=hq, Hk=hk, table_rows=cos.shape[-2], table_ld=_row_stride(cos),
+                           axes=axes, interleaved=bool(interleaved), pos_type=_POS_CODE[positions.dtype],
+                           dtype_x=_lib.dtype_code(q), dtype_cs=_lib.dtype_code(cos), inverse=inverse)
+    s.sections[:axes] = [int(c) for c in sections]
+    s.pos[:] = positions.stride()
+    if positions.shape[1] == 1:
+        s.pos[1] = 0
+    for x, rows_in, rows_out in ((q, s.q_in, s.q_out), (k, s.k_in, s.k_out)):
+        out = torch.empty_like(x)
+        assert x.stride(3) == 1 and out.stride(3) == 1
+        rows_in[:], rows_out[:] = x.stride()[:3], out.stride()[:3]
+    return dev, s
 
 
 def _launch(q, k, cos, sin, positions, sections, interleaved, inverse):
-    """(q_out, k_out): one launch over both."""
-    # shapes and strides are read once each (host time: a decode step's call is bound by it)
-    dev = _lib.require_device(q, k, cos, sin, positions)
-    qs, ks, cs, ps = q.shape, k.shape, cos.shape, positions.shape
-    assert len(qs) == 4 and len(ks) == 4, "q and k must be (bsz, n_heads, seq_len, head_dim)"
-    bsz, hq, seq_len, hd = qs
-    kb, hk, kt, kd = ks
-    assert kb == bsz and kt == seq_len and kd == hd, f"q and k differ: {tuple(qs)} and {tuple(ks)}"
-    dtype, table_dtype = q.dtype, cos.dtype
-    assert k.dtype == dtype, f"q and k have different dtypes: {dtype} and {k.dtype}"
-    assert sin.shape == cs and sin.dtype == table_dtype, "cos and sin must be alike"
-    assert (len(cs) == 2 or len(cs) == 3 and cs[0] == 1) and cs[-1] * 2 == hd, \
-        f"cos/sin must be (1, positions, head_dim/2); got {tuple(cs)}"
-    sec = _sections_arg(sections)
-    axes = len(sec)
-    pos_code = _POS_CODE.get(positions.dtype)
-    if pos_code is None:
-        raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-    assert len(ps) == 3 and ps[0] == axes and ps[2] == seq_len and (ps[1] == bsz or ps[1] == 1), \
-        f"positions must be ({axes}, {bsz} or 1, {seq_len}); got {tuple(ps)}"
-    pa, pb, pt = positions.stride()
-    if ps[1] == 1:
-        pb = 0
-    cst = cos.stride()
-    if cst[-1] != 1 or sin.stride() != cst:
-        cos, sin = cos.contiguous(), sin.contiguous()
-        cst = cos.stride()
-    qi, ki = q.stride(), k.stride()
-    if qi[3] != 1:
-        q = q.contiguous()
-        qi = q.stride()
-    if ki[3] != 1:
-        k = k.contiguous()
-        ki = k.stride()
+    """(q_out, k_out): one launch over both. A layout is checked once (host time: a decode step's call is bound by it)."""
+    sections = tuple(sections)
+    key = (q.shape, q.stride(), k.shape, k.stride(), cos.shape, cos.stride(), sin.shape, sin.stride(), positions.shape,
+           positions.stride(), q.dtype, k.dtype, cos.dtype, sin.dtype, positions.dtype, q.device, k.device, cos.device,
+           sin.device, positions.device, sections, interleaved, inverse)
+    known = _shapes.get(key)
+    if known is None:
+        again = [x if x.dim() == 0 or x.stride(-1) == 1 else x.contiguous() for x in (q, k, cos, sin)]
+        if cos.dim() >= 2 and cos.shape == sin.shape and not \
+                cos.shape[-1] <= _row_stride(again[2]) == _row_stride(again[3]):
+            again[2:] = again[2].contiguous(), again[3].contiguous()
+        if any(a is not b for a, b in zip(again, (q, k, cos, sin))):
+            return _launch(*again, positions, sections, interleaved, inverse)
+        known = _checked(q, k, cos, sin, positions, sections, interleaved, inverse)
+        if len(_shapes) >= 1024:
+            _shapes.clear()
+        _shapes[key] = known
+    dev, shape = known
     # empty_like keeps a dense input's layout and is contiguous for broadcast (zero-stride) ones
     q_out, k_out = torch.empty_like(q), torch.empty_like(k)
-    qo, ko = q_out.stride(), k_out.stride()
-    assert qo[3] == 1 and ko[3] == 1
-    _lib.call_on(dev, "hk_rope_axes", q_out.data_ptr(), q.data_ptr(), hq, qi[0], qi[1], qi[2], qo[0], qo[1], qo[2],
-                 k_out.data_ptr(), k.data_ptr(), hk, ki[0], ki[1], ki[2], ko[0], ko[1], ko[2],
-                 cos.data_ptr(), sin.data_ptr(), cs[-2], cst[-2], positions.data_ptr(), pos_code, pa, pb, pt, sec, axes,
-                 interleaved, bsz, seq_len, hd, _lib.dtype_code(q), _lib.dtype_code(cos), inverse)
+    _lib.call_on(dev, "hk_rope_axes", q_out.data_ptr(), q.data_ptr(), k_out.data_ptr(), k.data_ptr(), cos.data_ptr(),
+                 sin.data_ptr(), positions.data_ptr(), ctypes.addressof(shape))
     return q_out, k_out
 
 

@@ -152,21 +152,25 @@ int hk_rope_qk(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int64
 
 /* Multi-axis RoPE (no counterpart in the reference, whose tokens sit at the
  * positions 0..T-1 of one axis, rope.py:113-136): q (B, Hq, T, D) and
- * k (B, Hk, T, D) in one launch, strides as for hk_rope_qk. Pair i < D/2 turns
- * by row positions[a(i), b, t] of the cos/sin tables [table_rows, D/2] (last
- * dim contiguous, row stride table_ld), a(i) the axis that `sections` (host
- * array of `axes` counts, 1..4, sum D/2) gives it: runs of sections[a] pairs,
- * or with `interleaved` a = i mod axes while i < axes * sections[a], else 0.
- * positions: HK_I32 or HK_I64, element strides per axis, batch and token. A
+ * k (B, Hk, T, D) in one launch. Pair i < D/2 turns by row
+ * positions[a(i), b, t] of the cos/sin tables [table_rows, D/2] (last dim
+ * contiguous, row stride table_ld), a(i) the axis that `sections` (`axes`
+ * counts, 1..4, sum D/2) gives it: runs of sections[a] pairs, or with
+ * `interleaved` a = i mod axes while i < axes * sections[a], else 0. A
  * position outside [0, table_rows) gives NaN in its axis' pairs. inverse = 1
- * rotates back (the backward). out must not overlap in. */
-int hk_rope_axes(void* q_out, const void* q_in, int64_t Hq, int64_t q_in_sB, int64_t q_in_sH, int64_t q_in_sT,
-                 int64_t q_out_sB, int64_t q_out_sH, int64_t q_out_sT, void* k_out, const void* k_in, int64_t Hk,
-                 int64_t k_in_sB, int64_t k_in_sH, int64_t k_in_sT, int64_t k_out_sB, int64_t k_out_sH,
-                 int64_t k_out_sT, const void* cos, const void* sin, int64_t table_rows, int64_t table_ld,
-                 const void* positions, int pos_type, int64_t pos_sA, int64_t pos_sB, int64_t pos_sT,
-                 const int64_t* sections, int axes, int interleaved, int64_t B, int64_t T, int64_t D, int dtype_x,
-                 int dtype_cs, int inverse, hk_stream_t stream);
+ * rotates back (the backward). out must not overlap in.
+ * Strides are in elements: batch, head, token of the four row tensors (last
+ * dim contiguous), axis, batch, token of the positions (HK_I32 or HK_I64). */
+typedef struct {
+  int64_t B, T, D, Hq, Hk;
+  int64_t q_in[3], q_out[3], k_in[3], k_out[3], pos[3];
+  int64_t table_rows, table_ld;
+  int64_t sections[4];
+  int32_t axes, interleaved, pos_type, dtype_x, dtype_cs, inverse;
+} hk_rope_axes_shape;
+
+int hk_rope_axes(void* q_out, const void* q_in, void* k_out, const void* k_in, const void* cos, const void* sin,
+                 const void* positions, const hk_rope_axes_shape* shape, hk_stream_t stream);
 
 /* ----------------------------------------------------------------------- */
 /* SwiGLU                                                                  */

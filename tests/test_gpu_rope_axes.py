@@ -180,6 +180,26 @@ def test_one_gradient_only_and_differences():
     assert abs(change - (q.grad.double() * step.double()).sum()) <= 96 * 4 * 2.0 ** -22 * 9
 
 
+def test_table_layouts():
+    """Tables as rows only, cut from wider ones, laid out unlike each other, of one position, and one row for all."""
+    dev = gpu()
+    g = torch.Generator().manual_seed(10)
+    x = torch.randn(1, 2, 6, 16, generator=g)
+    cos, sin = oracle.rope_tables(16, 20, 10000.0)
+    pos = _positions(g, 2, 1, 6, 20)
+    wide = torch.cat((cos, sin), -1).to(dev)
+    flipped = sin.to(dev).transpose(1, 2).contiguous().transpose(1, 2)
+    for c, s in ((cos[0].to(dev), sin[0].to(dev)), (wide[..., :8], wide[..., 8:]), (cos.to(dev), wide[..., 8:]),
+                 (cos.to(dev), flipped), (cos[:, None].to(dev)[:, 0], sin.to(dev))):
+        for _ in range(2):
+            got = hilda_rope_axes(x.to(dev), x.to(dev), c, s, pos.to(dev), [4, 4])[0]
+            _check(got, *oracle.rope_axes_ref(x, cos[0], sin[0], pos, (4, 4)), torch.float32, "y")
+    one = torch.zeros(2, 1, 6, dtype=torch.int32)
+    for c, s in ((cos[:, :1], sin[:, :1]), (cos[:, :1].expand(1, 20, 8), sin[:, :1].expand(1, 20, 8))):
+        got = hilda_rope_axes(x.to(dev), x.to(dev), c.to(dev), s.to(dev), one.to(dev), (4, 4))[0]
+        _check(got, *oracle.rope_axes_ref(x, cos[0], sin[0], one, (4, 4)), torch.float32, "y")
+
+
 def test_empty_calls():
     dev = gpu()
     cos, sin = (t.to(dev) for t in oracle.rope_tables(16, 20, 10000.0))

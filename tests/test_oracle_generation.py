@@ -128,15 +128,16 @@ def test_rope_axes_refusals():
 
     def call(sections=(16, 24, 24), axes=None, interleaved=0, B=2, T=4, D=128, dtype=2, cs=0, pos=_lib.I64, stride=128,
              rows=100, ld=64, ptr=p):
-        sec = (ctypes.c_int64 * len(sections))(*sections)
-        return lib.hk_rope_axes(ptr, p, 2, stride, stride, stride, 1, 1, 1, p, p, 1, 1, 1, 1, 1, 1, 1, p, p, rows, ld, p,
-                                pos, 1, 1, 1, sec, len(sections) if axes is None else axes, interleaved, B, T, D, dtype,
-                                cs, 0, None)
+        s = _lib.RopeAxesShape(B=B, T=T, D=D, Hq=2, Hk=1, table_rows=rows, table_ld=ld, interleaved=interleaved,
+                               pos_type=pos, dtype_x=dtype, dtype_cs=cs, axes=len(sections) if axes is None else axes)
+        s.sections[:] = (tuple(sections) + (0, 0, 0, 0))[:4]
+        s.q_in[:] = (stride,) * 3
+        return lib.hk_rope_axes(ptr, p, p, p, p, p, p, ctypes.addressof(s), None)
 
     _einval(call(D=127), "even")
     _einval(call(sections=(16, 24, 23)), "sum to")
     _einval(call(sections=(70, -3, -3)), "negative")
-    _einval(call(sections=(16, 12, 12, 12, 12)), "axes")
+    _einval(call(axes=5), "axes")
     _einval(call(axes=0), "axes")
     # axis 1 of 2 over 64 pairs owns at most 32
     _einval(call(sections=(30, 34), interleaved=1), "interleaved section")
@@ -150,6 +151,7 @@ def test_rope_axes_refusals():
     _einval(call(B=-1), "invalid shape")
     _einval(call(ptr=None), "null")
     assert call(B=0, ptr=None) == 0
+    _einval(lib.hk_rope_axes(p, p, p, p, p, p, p, None, None), "null")
 
 
 @needs_lib
