@@ -64,23 +64,23 @@ struct Setting {
 };
 
 // Bins of logits, in descending order. fp32 and fp16: linear in max - x, with counts and masses. bf16: one bin for each
-// value of 2^-12 <= |x| < 2^8 (kSide of either sign), so a count is a mass, and three more that hold several: x >= 2^8,
-// |x| < 2^-12 and x <= -2^8.
+// value of 2^-16 <= |x| < 2^8 (kSide of either sign), so a count is a mass, and three more that hold several: x >= 2^8,
+// |x| < 2^-16 and x <= -2^8.
 template <typename T> struct Bins {
   static constexpr int kCount = 2048, kMasses = kCount;
   static constexpr bool kExact = false;
 };
 template <> struct Bins<__bf16> {
-  static constexpr int kSide = 20 * 128, kLowest = (127 - 12) << 7;  // kLowest: the bits of 2^-12
+  static constexpr int kSide = 24 * 128, kLowest = (127 - 16) << 7;  // kLowest: the bits of 2^-16
   static constexpr int kZero = kSide + 1, kUsed = 2 * kSide + 3;
-  static constexpr int kCount = 6144, kMasses = 4;  // (whole turns of the block; masses of the three)
+  static constexpr int kCount = 7168, kMasses = 4;  // (whole turns of the block; masses of the three)
   static constexpr bool kExact = true;
   static __device__ __forceinline__ int of(float v) {
     const int b = (int)f32_bits(v), sign = b >> 31;
     const int i = ::min(::max(((b >> 16) & 0x7fff) - kLowest + 1, 0), kSide + 1);
     return kZero - (i ^ sign) + sign;
   }
-  // of both bf16 values of a word, by packed 16-bit integers; `rank`: 0 for |x| < 2^-12, kSide + 1 for |x| >= 2^8
+  // of both bf16 values of a word, by packed 16-bit integers; `rank`: 0 for |x| < 2^-16, kSide + 1 for |x| >= 2^8
   typedef short Two __attribute__((ext_vector_type(2)));
   static __device__ __forceinline__ Two of_two(uint32_t w, Two* rank) {
     const Two sign = __builtin_bit_cast(Two, w) >> (short)15;
@@ -367,8 +367,13 @@ struct Start {
   }
 };
 
-// f(logit) for those of a pack that are in a bin of several values and above -inf. Few are, so the loop stays rolled: the
-// pack moves down by one logit a turn.
+// The pack's logits one place down.
+__device__ __forceinline__ void shift_down(Pack<__bf16, 8>& p) {
+#pragma unroll
+  for (int j = 0; j < 3; ++j) p.w[j] = __builtin_amdgcn_alignbit(p.w[j + 1], p.w[j], 16);
+  p.w[3] >>= 16;
+}
+// f(logit) for those of a pack that are in a bin of several values and above -inf. Few are, so the loop stays rolled.
 template <typename F>
 __device__ __forceinline__ void each_several(Pack<__bf16, 8> p, F&& f) {
   typedef Bins<__bf16> B;
@@ -376,57 +381,61 @@ __device__ __forceinline__ void each_several(Pack<__bf16, 8> p, F&& f) {
   for (int i = 0; i < 8; ++i) {
     const float v = bits_f32(p.w[0] << 16);
     if (B::several(B::of(v)) && v != -INFINITY) f(v);
-#pragma unroll
-    for (int j = 0; j < 3; ++j) p.w[j] = __builtin_amdgcn_alignbit(p.w[j + 1], p.w[j], 16);
-    p.w[3] >>= 16;
+    shift_down(p);
   }
 }
 
-// bf16: the masses of the bins that hold one value, 0 in the others, whose logits are looked at one by one.
+// bf16: the masses of the bins that hold one value, and NaN for the bins of several up to `reach` (0 after it).
 template <typename F>
-__device__ __forceinline__ void fill_table(double* table, F&& mass) {
+__device__ __forceinline__ void fill_table(double* table, int reach, F&& mass) {
   typedef Bins<__bf16> B;
 #pragma unroll 1
-  for (int b = threadIdx.x; b < B::kUsed; b += kLanes) table[b] = B::several(b) ? 0.0 : mass(B::value(b));
+  for (int b = threadIdx.x; b < B::kUsed; b += kLanes)
+    table[b] = b > reach ? 0.0 : B::several(b) ? (double)__builtin_nanf("") : mass(B::value(b));
   __syncthreads();
 }
-// The sum of the table's masses over a pack, and of `mass` over its few logits of the other bins; 0 if no logit of the
-// wave comes up to the bin `reach`.
+// The sum of the masses of a pack's logits: from the table, and by `mass` where that has NaN; 0 if no logit of the wave
+// comes up to the bin `reach`.
 template <typename F>
 __device__ __forceinline__ double sum_table(const double* table, const Pack<__bf16, 8>& p, int reach, F&& mass) {
   typedef Bins<__bf16> B;
-  B::Two bins[4], least = (B::Two)((short)B::kUsed), low = (B::Two)((short)B::kSide), high = (B::Two)((short)0);
+  B::Two bins[4], least = (B::Two)((short)B::kUsed), rank;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    B::Two rank;
-    bins[j] = B::of_two(p.w[j], &rank);
-    least = __builtin_elementwise_min(least, bins[j]);
-    low = __builtin_elementwise_min(low, rank);
-    high = __builtin_elementwise_max(high, rank);
-  }
+  for (int j = 0; j < 4; ++j) bins[j] = B::of_two(p.w[j], &rank), least = __builtin_elementwise_min(least, bins[j]);
+  if (!__any(min(least.x, least.y) <= reach)) return 0.0;
   double s0 = 0.0, s1 = 0.0;
-  if (__any(min(least.x, least.y) <= reach)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s0 += table[bins[j].x], s1 += table[bins[j].y];
-    if (min(low.x, low.y) == 0 || max(high.x, high.y) > B::kSide) each_several(p, [&](float v) { s0 += mass(v); });
+  for (int j = 0; j < 4; ++j) s0 += table[bins[j].x], s1 += table[bins[j].y];
+  s0 += s1;
+  if (s0 != s0) {  // few: the loop stays rolled, the pack moves down by one logit a turn
+    Pack<__bf16, 8> q = p;
+    s0 = 0.0;
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const float v = bits_f32(q.w[0] << 16);
+      const double e = table[B::of(v)];
+      if (e == e) s0 += e;
+      else if (v != -INFINITY) s0 += mass(v);
+      shift_down(q);
+    }
   }
-  return s0 + s1;
+  return s0;
 }
 
 // ---- scan -------------------------------------------------------------------
+// The maximum and the sum of e^(z - max) of a block's runs, in its first wave; quarters: where the maxima of each run's
+// quarters go, or null.
+struct ScanShared {
+  float m[kWaves], z[kWaves];
+};
 template <typename T>
-__global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
+__device__ __forceinline__ void scan_block(const T* x, const SampleArgs& g, int part, int split, float c, float* quarters,
+                                           ScanShared& sh, float* max, float* sum) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ float sm[kWaves], sz[kWaves];
-  const int64_t row = blockIdx.x / g.split;
-  const int part = blockIdx.x % g.split;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const Asked a = asked(g, row);
-  const T* x = static_cast<const T*>(g.logits) + row * g.ld;
-  const float c = (float)a.k;
   float m = -INFINITY, z = 0.f, rm = -INFINITY;  // rm: of the run
   each_run(
-      x, g.cols, g.run_cols, g.runs, part * kWaves + wave, g.split * kWaves,
+      x, g.cols, g.run_cols, g.runs, part * kWaves + wave, split * kWaves,
       [&](const Pack<T, VEC>& p) {
         float v[VEC];
         unpack(p, v);
@@ -441,13 +450,13 @@ __global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
         m = n;
       },
       [&](int run) {
-        if (!a.by_k) return;
+        if (!quarters) return;
         float q = rm;
         q = fmaxf(q, dpp_move<dpp::kXor1>(q, q));
         q = fmaxf(q, dpp_move<dpp::kXor2>(q, q));
         q = fmaxf(q, dpp_move<dpp::kHalfMirror>(q, q));
         q = fmaxf(q, dpp_move<dpp::kMirror>(q, q));
-        if (lane % 16 == 0) g.quarters[(row * g.runs + run) * 4 + lane / 16] = q;
+        if (lane % 16 == 0) quarters[run * 4 + lane / 16] = q;
         rm = -INFINITY;
       });
   {
@@ -455,14 +464,23 @@ __global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
     z = wave_sum(m == -INFINITY ? z : z * exp2_fast((m - ref) * c));
     m = wm;
   }
-  if (lane == 0) sm[wave] = m, sz[wave] = z;
+  if (lane == 0) sh.m[wave] = m, sh.z[wave] = z;
   __syncthreads();
-  if (wave > 0) return;
-  m = lane < kWaves ? sm[lane] : -INFINITY;
-  z = lane < kWaves ? sz[lane] : 0.f;
-  const float bm = wave_max(m);
-  z = wave_sum(m == -INFINITY ? z : z * exp2_fast((m - bm) * c));
-  if (lane == 0) g.part_max[blockIdx.x] = bm, g.part_sum[blockIdx.x] = z;
+  m = lane < kWaves ? sh.m[lane] : -INFINITY;
+  z = lane < kWaves ? sh.z[lane] : 0.f;
+  *max = wave_max(m);
+  *sum = wave_sum(m == -INFINITY ? z : z * exp2_fast((m - *max) * c));
+}
+
+template <typename T>
+__global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
+  __shared__ ScanShared sh;
+  const int64_t row = blockIdx.x / g.split;
+  const Asked a = asked(g, row);
+  float max, sum;
+  scan_block(static_cast<const T*>(g.logits) + row * g.ld, g, (int)(blockIdx.x % g.split), g.split, (float)a.k,
+             a.by_k ? g.quarters + row * g.runs * 4 : nullptr, sh, &max, &sum);
+  if (threadIdx.x == 0) g.part_max[blockIdx.x] = max, g.part_sum[blockIdx.x] = sum;
 }
 
 // A call without filters: the mass of each run, and its maximum.
@@ -481,7 +499,7 @@ __global__ __launch_bounds__(kLanes) void sample_open_kernel(SampleArgs g) {
   const int first = part * kWaves + wave, waves = g.split * kWaves;
   const bool use_table = kTable && a.temp >= 0.5 && g.runs * (g.run_cols / 512) > 8 * waves;
   if constexpr (kTable) {
-    if (use_table) fill_table(table, [&](float v) { return exp2_product((double)v, a.k); });
+    if (use_table) fill_table(table, Bins<T>::kUsed, [&](float v) { return exp2_product((double)v, a.k); });
   }
   // m: this lane's maximum in the run, and (without the table) the logit whose mass is 1
   float m = -INFINITY;
@@ -610,14 +628,14 @@ struct Row {
   float bin_step;   // linear bins: bins / (kRange T)
   double magic;
 
-  __device__ __forceinline__ Row(const SampleArgs& g, int64_t row, const Start& st)
+  __device__ __forceinline__ Row(const SampleArgs& g, int64_t row, const Asked& a, float max_)
       : x(static_cast<const T*>(g.logits) + row * g.ld),
         cols(g.cols),
         run_cols(g.run_cols),
         runs(g.runs),
-        max(st.max),
-        k(st.a.k),
-        bin_step((float)(B::kCount / kRange * kLn2D * st.a.k)),
+        max(max_),
+        k(a.k),
+        bin_step((float)(B::kCount / kRange * kLn2D * a.k)),
         magic(g.magic) {}
   __device__ __forceinline__ double mass(float v) const { return exp2_product((double)v - (double)max, k); }
   __device__ __forceinline__ u64 fixed(double e) const {
@@ -720,8 +738,8 @@ struct Row {
         *value = B::value(bin);
         return true;
       }
-      *khi = bin == 0 ? key_of<T>(max) : bin == B::kZero ? key_of<T>(0x1p-12f) : key_of<T>(-0x1p8f);
-      *klo = bin == 0 ? key_of<T>(0x1p8f) : bin == B::kZero ? key_of<T>(-0x1p-12f) : 0;
+      *khi = bin == 0 ? key_of<T>(max) : bin == B::kZero ? key_of<T>(0x1p-16f) : key_of<T>(-0x1p8f);
+      *klo = bin == 0 ? key_of<T>(0x1p8f) : bin == B::kZero ? key_of<T>(-0x1p-16f) : 0;
       return false;
     } else {
       // with the roundings of bin_of to spare
@@ -765,7 +783,7 @@ struct Row {
         for (int i = threadIdx.x; i < kFineBins; i += kLanes) sh.fine.mass[i] = 0, sh.fine.count[i] = 0, sh.fine.key[i] = 0;
         __syncthreads();
         // one block reads the row: it needs many loads on their way, and finds few logits
-        constexpr int kAhead = 6, kStep = kLanes * VEC;
+        constexpr int kAhead = B::kExact ? 2 : 6, kStep = kLanes * VEC;
 #pragma unroll 1
         for (int c0 = (int)threadIdx.x * VEC; c0 < cols; c0 += kAhead * kStep) {
           Pack<T, VEC> p[kAhead];
@@ -826,6 +844,9 @@ struct Row {
   __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a) const {
     const Share<B::kCount> share(
         sh.hist.count, [&](int b, uint32_t c) { return a.by_p ? mass_of_bin(sh.hist, b, c) : 0; }, sh);
+    return find(sh, a, share);
+  }
+  __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a, const Share<B::kCount>& share) const {
     u64 total = share.all_mass;
     Cut cut = {INFINITY, 0, 0, 0};
     // by count, then by mass of what that kept
@@ -882,7 +903,7 @@ __global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
   const int64_t row = blockIdx.x / g.split;
   const Start st(g, row, false);
   if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
-  const Row<T> r(g, row, st);
+  const Row<T> r(g, row, st.a, st.max);
   r.fill(sh.hist, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, st.a, sh), st.a.by_p);
   if constexpr (WHOLE) {
     const Cut cut = r.find(sh, st.a);
@@ -919,7 +940,7 @@ __global__ __launch_bounds__(kLanes) void sample_cut_kernel(SampleArgs g) {
   const int64_t row = blockIdx.x;
   const Start st(g, row, false);
   if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
-  const Row<T> r(g, row, st);
+  const Row<T> r(g, row, st.a, st.max);
   const Hist<T>* from = static_cast<const Hist<T>*>(g.hist) + row * g.split;
 #pragma unroll 1
   for (int i = 4 * threadIdx.x; i < Bins<T>::kCount; i += 4 * kLanes)
@@ -933,6 +954,127 @@ __global__ __launch_bounds__(kLanes) void sample_cut_kernel(SampleArgs g) {
   if (threadIdx.x == 0) g.cuts[row] = cut;
 }
 
+// ---- count: bf16's scan, hist and cut -----------------------------------------
+// bf16 bins do not depend on the maximum, so the row's first reading fills them; the maximum is the first bin with a
+// count, and the sum of e^(z - max) that of the bins' masses. What the bins cannot tell (|x| >= 2^8, NaN, a maximum of
+// |x| < 2^-16, or such x at a temperature that takes their masses far from 1) sets a flag, and the row's cut is made by
+// scan and hist in one block.
+constexpr double kTinyTemp = 0x1p-4;
+constexpr int kFlag = 3;  // the place of h.mass that counts what was flagged
+struct CountShared : CutShared<__bf16> {
+  ScanShared scan;
+  int first[kWaves];
+};
+
+// Counts one block's runs into h. h.mass[1] sums 2^(x k) of |x| < 2^-16.
+__device__ __forceinline__ void count_block(Hist<__bf16>& h, const SampleArgs& g, const __bf16* x, const Asked& a, int part) {
+  typedef Bins<__bf16> B;
+  for (int i = threadIdx.x; i < B::kCount; i += kLanes) h.count[i] = 0;
+  if (threadIdx.x < B::kMasses) h.mass[threadIdx.x] = 0;
+  __syncthreads();
+  constexpr int kLow = B::kUsed - 1;
+  uint32_t low = 0;
+  each_run(
+      x, g.cols, g.run_cols, g.runs, part * kWaves + (int)threadIdx.x / kWave, g.split * kWaves,
+      [&](const Pack<__bf16, 8>& p) {
+        B::Two least = (B::Two)((short)B::kSide), most = (B::Two)((short)0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          B::Two rank;
+          const B::Two b = B::of_two(p.w[j], &rank);
+          least = __builtin_elementwise_min(least, rank);
+          most = __builtin_elementwise_max(most, rank);
+          if (b.x < kLow) atomicAdd(&h.count[b.x], 1u);
+          else ++low;
+          if (b.y < kLow) atomicAdd(&h.count[b.y], 1u);
+          else ++low;
+        }
+        if (min(least.x, least.y) == 0 || max(most.x, most.y) > B::kSide)
+          each_several(p, [&](float v) {
+            if (fabsf(v) < 1.f && a.temp >= kTinyTemp)
+              atomicAdd(&h.mass[1], __builtin_bit_cast(u64, exp2_product((double)v, a.k) + g.magic) & 0xfffffffffffffull);
+            else
+              atomicAdd(&h.mass[kFlag], 1ull);
+          });
+      },
+      [](int) {});
+  low = wave_total(low);
+  if (threadIdx.x % kWave == 0) atomicAdd(&h.count[kLow], low);
+}
+
+// The row's maximum, sum and cut from the counts of all its columns.
+__device__ __forceinline__ void cut_counted(CountShared& sh, const SampleArgs& g, int64_t row, const Asked& a) {
+  typedef Bins<__bf16> B;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const __bf16* x = static_cast<const __bf16*>(g.logits) + row * g.ld;
+  __syncthreads();
+  // the first bin with a count
+  constexpr int kEach = B::kCount / kLanes;
+  int first = B::kCount;
+#pragma unroll
+  for (int i = kEach - 1; i >= 0; --i)
+    if (sh.hist.count[kEach * threadIdx.x + i]) first = kEach * threadIdx.x + i;
+  const u64 some = __ballot(first < B::kCount);
+  if (lane == 0) sh.first[wave] = B::kCount;
+  if (some && lane == __builtin_ctzll(some)) sh.first[wave] = first;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) first = min(first, sh.first[i]);
+  float max = B::value(first), sum = 0.f;
+  Cut cut = {-INFINITY, 0xffffffffu, 0, 0xffffffffu};
+  const bool cuts = a.by_k || a.by_p, again = sh.hist.mass[kFlag] || B::several(first);
+  if (again) scan_block(x, g, 0, 1, (float)a.k, nullptr, sh.scan, &max, &sum);
+  const Row<__bf16> r(g, row, a, max);
+  const bool ok = !again || (sum > 0.f && sum < INFINITY && max < INFINITY);
+  __syncthreads();
+  if (again && ok && cuts) r.fill(sh.hist, 0, 1, -INFINITY, true);
+  if (!again && threadIdx.x == 0)  // in terms of the maximum from here on
+    sh.hist.mass[1] = (u64)((double)sh.hist.mass[1] * exp2_product(-(double)max, a.k) + 0.5);
+  if (ok && (cuts || !again)) {
+    const Share<B::kCount> share(
+        sh.hist.count, [&](int b, uint32_t c) { return r.mass_of_bin(sh.hist, b, c); }, sh);
+    if (!again) sum = (float)((double)share.all_mass / (double)r.fixed(1.0));
+    if (cuts) cut = r.find(sh, a, share);
+  }
+  if (threadIdx.x < g.split) {
+    g.part_max[row * g.split + threadIdx.x] = threadIdx.x == 0 ? max : -INFINITY;
+    g.part_sum[row * g.split + threadIdx.x] = threadIdx.x == 0 ? sum : 0.f;
+  }
+  if (threadIdx.x == 0) g.cuts[row] = cut;
+}
+
+template <bool WHOLE>
+__global__ __launch_bounds__(kLanes) void sample_count_kernel(SampleArgs g) {
+  __shared__ __align__(16) typename std::conditional<WHOLE, CountShared, HistShared<__bf16>>::type sh;
+  const int64_t row = blockIdx.x / g.split;
+  const Asked a = asked(g, row);
+  count_block(sh.hist, g, static_cast<const __bf16*>(g.logits) + row * g.ld, a, (int)(blockIdx.x % g.split));
+  if constexpr (WHOLE) {
+    cut_counted(sh, g, row, a);
+  } else {
+    __syncthreads();
+    u32x4* to = reinterpret_cast<u32x4*>(static_cast<Hist<__bf16>*>(g.hist) + blockIdx.x);
+    for (int i = threadIdx.x; i < (int)(sizeof(Hist<__bf16>) / 16); i += kLanes)
+      to[i] = reinterpret_cast<const u32x4*>(&sh.hist)[i];
+  }
+}
+
+// (split > 1)
+__global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) {
+  typedef Bins<__bf16> B;
+  __shared__ __align__(16) CountShared sh;
+  const int64_t row = blockIdx.x;
+  const Hist<__bf16>* from = static_cast<const Hist<__bf16>*>(g.hist) + row * g.split;
+  const Asked a = asked(g, row);
+#pragma unroll 1
+  for (int i = 4 * threadIdx.x; i < B::kCount; i += 4 * kLanes)
+    *reinterpret_cast<u32x4*>(&sh.hist.count[i]) =
+        sum_parts<u32x4>((const char*)&from->count[i], sizeof(Hist<__bf16>), g.split);
+  if (threadIdx.x < B::kMasses) sh.hist.mass[threadIdx.x] =
+      sum_parts<u64>((const char*)&from->mass[threadIdx.x], sizeof(Hist<__bf16>), g.split);
+  cut_counted(sh, g, row, a);
+}
+
 // ---- mass -------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
@@ -944,7 +1086,7 @@ __global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const Start st(g, row, true);
   if (!st.ok) return;
-  const Row<T> r(g, row, st);
+  const Row<T> r(g, row, st.a, st.max);
   const Cut cut = st.cut;
   const bool all_ties = cut.ties >= cut.equal;
   auto kept = [&](float v) { return all_ties ? v >= cut.x : v > cut.x; };
@@ -967,8 +1109,8 @@ __global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
   if constexpr (kTable) {
     // few are kept: the table costs more than their polynomials (2 us; 1 in 64 of 38000 logits a block 0.6)
     if (cut.count > (uint32_t)g.cols / 64) {
-      fill_table(table, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
       const int reach = Bins<T>::of(cut.x);
+      fill_table(table, reach, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
       each_run(
           r.x, g.cols, g.run_cols, g.runs, first, waves,
           [&](const Pack<T, VEC>& p) {
@@ -1039,7 +1181,7 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
     return;
   }
   const float max = st.max;
-  const Row<T> r(g, row, st);
+  const Row<T> r(g, row, st.a, st.max);
   const Cut cut = g.open ? Cut{-INFINITY, 0xffffffffu, 0, 0} : st.cut;
   const bool all_ties = cut.ties >= cut.equal;
   const double each = all_ties ? 0.0 : r.mass(cut.x);
@@ -1244,16 +1386,35 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
     using T = decltype(tag);
     const hipStream_t st = (hipStream_t)stream;
     const dim3 parts((unsigned)(rows * split)), each((unsigned)rows);
-    if (masses) hipLaunchKernelGGL((sample_scan_kernel<T>), parts, dim3(kLanes), 0, st, g);
-    else hipLaunchKernelGGL((sample_open_kernel<T>), parts, dim3(kLanes), 0, st, g);
-    if (const int rc = check_launch("sample_scan_kernel")) return rc;
-    if (cuts) {
-      if (split == 1) hipLaunchKernelGGL((sample_hist_kernel<T, true>), parts, dim3(kLanes), 0, st, g);
-      else hipLaunchKernelGGL((sample_hist_kernel<T, false>), parts, dim3(kLanes), 0, st, g);
-      if (const int rc = check_launch("sample_hist_kernel")) return rc;
-      if (split > 1) {
-        hipLaunchKernelGGL((sample_cut_kernel<T>), each, dim3(kLanes), 0, st, g);
-        if (const int rc = check_launch("sample_cut_kernel")) return rc;
+    if constexpr (Bins<T>::kExact) {
+      if (cuts) {
+        if (split == 1) {
+          hipLaunchKernelGGL((sample_count_kernel<true>), parts, dim3(kLanes), 0, st, g);
+          if (const int rc = check_launch("sample_count_kernel")) return rc;
+        } else {
+          hipLaunchKernelGGL((sample_count_kernel<false>), parts, dim3(kLanes), 0, st, g);
+          if (const int rc = check_launch("sample_count_kernel")) return rc;
+          hipLaunchKernelGGL(sample_count_cut_kernel, each, dim3(kLanes), 0, st, g);
+          if (const int rc = check_launch("sample_count_cut_kernel")) return rc;
+        }
+      }
+    }
+    if (!masses) {
+      hipLaunchKernelGGL((sample_open_kernel<T>), parts, dim3(kLanes), 0, st, g);
+      if (const int rc = check_launch("sample_open_kernel")) return rc;
+    } else if (!Bins<T>::kExact || !cuts) {
+      hipLaunchKernelGGL((sample_scan_kernel<T>), parts, dim3(kLanes), 0, st, g);
+      if (const int rc = check_launch("sample_scan_kernel")) return rc;
+    }
+    if constexpr (!Bins<T>::kExact) {
+      if (cuts) {
+        if (split == 1) hipLaunchKernelGGL((sample_hist_kernel<T, true>), parts, dim3(kLanes), 0, st, g);
+        else hipLaunchKernelGGL((sample_hist_kernel<T, false>), parts, dim3(kLanes), 0, st, g);
+        if (const int rc = check_launch("sample_hist_kernel")) return rc;
+        if (split > 1) {
+          hipLaunchKernelGGL((sample_cut_kernel<T>), each, dim3(kLanes), 0, st, g);
+          if (const int rc = check_launch("sample_cut_kernel")) return rc;
+        }
       }
     }
     if (masses) {
