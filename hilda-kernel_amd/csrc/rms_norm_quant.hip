@@ -373,6 +373,7 @@ int hk_rms_norm_quant_fwd(void* q, float* scale, void* s, float* rstd, const voi
       constexpr bool ADD = decltype(add_c)::value, GROUPS = decltype(groups_c)::value;
       Geom g;
       if (!choose_geom(cols, VEC, ADD, &g)) {
+        HK_REQUIRE(rows < (1LL << 32) / kStreamLanes, "rows=%lld too many for one launch", (long long)rows);
         hipLaunchKernelGGL((rmsnorm_quant_stream_kernel<T, W, ADD, GROUPS>), dim3((unsigned)rows), dim3(kStreamLanes),
                            0, st, (uint8_t*)q, scale, (T*)s, rstd, (const T*)x, (const T*)r, (const W*)w, (int)cols,
                            ld, group_lanes, eps);
@@ -380,6 +381,7 @@ int hk_rms_norm_quant_fwd(void* q, float* scale, void* s, float* rstd, const voi
       }
       const int rows_block = std::max(1, 4 / g.wpr), block = rows_block * g.wpr * kWave;
       const int64_t grid = cdiv(rows, (int64_t)rows_block);
+      HK_REQUIRE(grid < (1LL << 32) / block, "rows=%lld too many for one launch", (long long)rows);
       auto launch = [&](auto nch_c, auto lb_c) {
         constexpr int NCH = decltype(nch_c)::value, LB = decltype(lb_c)::value;
         hipLaunchKernelGGL((rmsnorm_quant_kernel<T, W, NCH, ADD, GROUPS, LB>), dim3((unsigned)grid), dim3(block), 0, st,

@@ -262,6 +262,7 @@ int hk_rope_axes(void* q_out, const void* q_in, void* k_out, const void* k_in, c
         g.tokens_block = tb;
         g.slots = (uint32_t)std::min<int64_t>(heads, per_block / tb);
         const int64_t blocks = cdiv(g.tokens, (int64_t)tb);
+        HK_REQUIRE(blocks < (1LL << 32) / kThreads, "B * T = %lld too many for one launch", (long long)g.tokens);
         const dim3 grid((unsigned)blocks, (unsigned)cdiv((int64_t)g.chunks, (int64_t)g.lanes));
         auto go = [&](auto tp, auto order) {
           using TP = typename decltype(tp)::type;

@@ -14,18 +14,30 @@
 // Nothing is sorted. The kept set is a threshold x* and a number of ties at
 // x* that are kept (the first ones by index), found by selection. A row is cut
 // into runs of 512 to 2048 columns, its runs are dealt to the waves of a few
-// blocks, and up to five launches follow each other (the later ones read the
-// row from the Infinity Cache):
-//   scan  max and log-sum-exp (fp32); in a call without filters (open) the
-//         fp64 mass of each run instead
-//   hist  counts, and for top-p masses, in kBins bins linear in max - x
-//   cut   the bins of a row's blocks together; the bin that holds the cut; if
-//         several values may lie in it, the same over ranges of ordered keys,
-//         11 bits at a time, until one is left: x* and how many ties are kept
-//   mass  the kept mass of each run
-//   pick  the run that u * total falls into, and the token inside it
-// A call whose settings are numbers launches those it needs: open and pick
-// without filters, scan, mass and pick with min-p alone.
+// blocks, and a few launches follow each other (the first reads the row from
+// HBM, the later ones from the Infinity Cache):
+//   no filter       open, pick
+//   min-p alone     scan, mass, pick
+//   top-k or top-p  bf16: count, cut, mass, pick
+//                   fp16, fp32: scan, hist, cut, mass, pick
+// (a setting that comes row by row may be any of its values)
+//   open   the fp64 mass and the maximum of each run
+//   scan   max and log-sum-exp (fp32)
+//   hist   counts, and for top-p masses, in bins linear in max - x
+//   count  counts in bins of one bf16 value each, which give the maximum, the
+//          sum and every mass
+//   cut    the bins of a row's blocks together; the bin that holds the cut; if
+//          several values may lie in it, the same over ranges of ordered keys,
+//          11 bits at a time, until one is left: x* and how many ties are kept.
+//          With one block a row this ends the launch before.
+//   mass   the kept mass of each run
+//   pick   the run that u * total falls into, and the token inside it
+//
+// What bounds it: the first pass of 256 rows of 151936 bf16 logits (78 MB) runs
+// at HBM's rate (scan 15 us); the bins' LDS atomics (count 23 us) and the mass
+// table's LDS gathers (mass 34 us, 33 cycles a wave's) are LDS-bound, cut and
+// pick (11 and 7 us) chains of latencies. 77 us in all with top-p, 34 without
+// filters; few rows are bound by those chains, 4 to 14 us a launch.
 //
 // Masses are fp64: with 32-bit ones the running sums of a flat row of 1e5
 // tokens (steps of 1e-5 of the total) would be off by a percent of a step, and
@@ -564,6 +576,8 @@ struct Fine {
 // What the bins of a block's columns need, and what finding a cut needs beside.
 template <typename T> struct HistShared {
   Hist<T> hist;
+};
+struct BoundShared {
   float groups[kGroups], best[kGroups / kWave];
   int reach[kLanes];
 };
@@ -658,7 +672,8 @@ struct Row {
     }
   }
 
-  // Adds the runs of one block (part of split) to h; logits below `least` are left out.
+  // Adds the runs of one block (part of split) to h; logits below `least` are left out (bf16: none is, and masses are
+  // those of the bins of several).
   __device__ __forceinline__ void fill(Hist<T>& h, int part, int split, float least, bool masses) const {
     for (int i = threadIdx.x; i < B::kCount; i += kLanes) h.count[i] = 0;
     for (int i = threadIdx.x; i < B::kMasses; i += kLanes) h.mass[i] = 0;
@@ -668,8 +683,6 @@ struct Row {
     const int first = part * kWaves + (int)threadIdx.x / kWave, waves = split * kWaves;
     if constexpr (B::kExact) {
       constexpr int kLow = Bins<__bf16>::kUsed - 1;
-      // (what is left out counts as low: the k-th logit lies above)
-      const int reach = least == -INFINITY ? kLow - 1 : ::min(kLow - 1, B::of(least));
       each_run(
           x, cols, run_cols, runs, first, waves,
           [&](const Pack<T, VEC>& p) {
@@ -680,12 +693,12 @@ struct Row {
               const typename B::Two b = B::of_two(p.w[j], &rank);
               low2 = __builtin_elementwise_min(low2, rank);
               high2 = __builtin_elementwise_max(high2, rank);
-              if (b.x <= reach) atomicAdd(&h.count[b.x], 1u);
+              if (b.x < kLow) atomicAdd(&h.count[b.x], 1u);
               else ++low;
-              if (b.y <= reach) atomicAdd(&h.count[b.y], 1u);
+              if (b.y < kLow) atomicAdd(&h.count[b.y], 1u);
               else ++low;
             }
-            if (masses && (::min(low2.x, low2.y) == 0 || ::max(high2.x, high2.y) > B::kSide))
+            if (::min(low2.x, low2.y) == 0 || ::max(high2.x, high2.y) > B::kSide)
               each_several(p, [&](float v) { atomicAdd(&h.mass[B::slot(B::of(v))], fixed(mass(v))); });
           },
           [](int) {});
@@ -866,8 +879,7 @@ struct Row {
 // A lower bound of the k-th largest logit, k <= kGroups: the k-th largest of the maxima of kGroups disjoint sets of
 // columns (each of those k is a logit of its own), put together from the scan's. Its value is the largest that k of them
 // reach; four threads count for each.
-template <typename S>
-__device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row, const Asked& a, S& sh) {
+__device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row, const Asked& a, BoundShared& sh) {
   static_assert(kLanes == 4 * kGroups, "four threads a group");
   const int n = 4 * g.runs, i = threadIdx.x % kGroups, part = threadIdx.x / kGroups;
   if (!a.by_k || a.top_k > min(n, kGroups)) return -INFINITY;
@@ -900,11 +912,12 @@ __device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
   __shared__ __align__(16) typename std::conditional<WHOLE, CutShared<T>, HistShared<T>>::type sh;
+  __shared__ BoundShared bound;
   const int64_t row = blockIdx.x / g.split;
   const Start st(g, row, false);
   if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
   const Row<T> r(g, row, st.a, st.max);
-  r.fill(sh.hist, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, st.a, sh), st.a.by_p);
+  r.fill(sh.hist, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, st.a, bound), st.a.by_p);
   if constexpr (WHOLE) {
     const Cut cut = r.find(sh, st.a);
     if (threadIdx.x == 0) g.cuts[row] = cut;
@@ -1027,7 +1040,7 @@ __device__ __forceinline__ void cut_counted(CountShared& sh, const SampleArgs& g
   const Row<__bf16> r(g, row, a, max);
   const bool ok = !again || (sum > 0.f && sum < INFINITY && max < INFINITY);
   __syncthreads();
-  if (again && ok && cuts) r.fill(sh.hist, 0, 1, -INFINITY, true);
+  if (again && ok && cuts) r.fill(sh.hist, 0, 1, -INFINITY, a.by_p);
   if (!again && threadIdx.x == 0)  // in terms of the maximum from here on
     sh.hist.mass[1] = (u64)((double)sh.hist.mass[1] * exp2_product(-(double)max, a.k) + 0.5);
   if (ok && (cuts || !again)) {
@@ -1346,7 +1359,7 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   const int cus = cu_count(dev);
   const Shape shape = shape_of(rows, cols, cus > 0 ? cus : 256);
   const int split = (int)shape.split;
-  HK_REQUIRE(rows * split < (1LL << 31), "rows=%lld too large", (long long)rows);
+  HK_REQUIRE(rows * split < (1LL << 32) / kLanes, "rows=%lld too many for one launch", (long long)rows);
   const bool cuts = top_k_rows || (top_k > 0 && top_k < cols) || top_p_rows || top_p < 1;
   const bool masses = cuts || min_p_rows || min_p > 0;
   const Layout l = layout_of(rows, shape, cuts, dtype == kBF16);

@@ -97,19 +97,20 @@ def rope_axes_backward(dq, dk, cos, sin, positions, sections, interleaved=False)
 
 
 class HildaRopeAxesFunction(torch.autograd.Function):
-    """Autograd wrapper: q, k = HildaRopeAxesFunction.apply(q, k, cos, sin, positions, sections, interleaved)."""
+    """Autograd wrapper: q, k = HildaRopeAxesFunction.apply(q, k, cos, sin, positions, sections, interleaved). The
+    rotation is linear, so its backward is one of the other sense, and can be differentiated again."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, sections, interleaved):
+    def forward(ctx, q, k, cos, sin, positions, sections, interleaved=False, inverse=False):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.sections, ctx.interleaved = sections, interleaved
-        return rope_axes_forward(q, k, cos, sin, positions, sections, interleaved)
+        ctx.args = sections, interleaved, not inverse
+        return _launch(q, k, cos, sin, positions, sections, interleaved, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        cos, sin, positions = ctx.saved_tensors
-        dq, dk = rope_axes_backward(dq, dk, cos, sin, positions, ctx.sections, ctx.interleaved)
-        return dq, dk, None, None, None, None, None
+        call = HildaRopeAxesFunction.apply if torch.is_grad_enabled() else _launch
+        dq, dk = call(dq, dk, *ctx.saved_tensors, *ctx.args)
+        return dq, dk, None, None, None, None, None, None
 
 
 def hilda_rope_axes(q, k, cos, sin, positions, sections, interleaved=False):

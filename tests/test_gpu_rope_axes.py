@@ -180,6 +180,22 @@ def test_one_gradient_only_and_differences():
     assert abs(change - (q.grad.double() * step.double()).sum()) <= 96 * 4 * 2.0 ** -22 * 9
 
 
+def test_gradient_of_the_gradient():
+    """Linear: the second derivative along v of <w, y(q)^2> / 2 is the rotation of v back and forth, v itself."""
+    dev = gpu()
+    g = torch.Generator().manual_seed(11)
+    q = torch.randn(1, 2, 3, 16, generator=g).to(dev).requires_grad_()
+    k = torch.randn(1, 1, 3, 16, generator=g).to(dev)
+    cos, sin = (t.to(dev) for t in oracle.rope_tables(16, 20, 10000.0))
+    pos = _positions(g, 2, 1, 3, 20).to(dev)
+    y = hilda_rope_axes(q, k, cos, sin, pos, (4, 4))[0]
+    first = torch.autograd.grad((y * y).sum() / 2, q, create_graph=True)[0]
+    v = torch.randn(1, 2, 3, 16, generator=g).to(dev)
+    second = torch.autograd.grad(first, q, v)[0]
+    # two rotations, each within 3 * 2^-24 of terms of size |v|, and cos^2 + sin^2 of fp32 tables
+    assert (second - v).abs().max() <= 8 * 2.0 ** -23 * v.abs().max() * 2
+
+
 def test_table_layouts():
     """Tables as rows only, cut from wider ones, laid out unlike each other, of one position, and one row for all."""
     dev = gpu()

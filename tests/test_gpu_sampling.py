@@ -279,3 +279,37 @@ def test_workspace_is_checked():
         assert (status == 0) == ok
     assert "workspace too small" in _lib.last_error()
     assert ids.tolist() == [0] * 4
+
+
+@pytest.mark.parametrize("rows", [1, 5, 600, 1100])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ways_a_call_is_cut_up(rows, dtype):
+    """Few rows are split over many blocks, many rows take one block each, with runs of 512 to 2048 columns."""
+    V = 40011 if rows <= 5 else 2500
+    x, u, g = _rows(rows, V, dtype, seed=rows)
+    _check(x, u, temperature=0.8)
+    _check(x, u, temperature=0.8, top_k=60, top_p=0.9)
+    _check(x, u, temperature=0.4, top_p=0.97, min_p=0.001)
+
+
+def test_bf16_values_outside_the_bins_of_one_value():
+    """bf16 logits of 2^8 and more, below 2^-16, and rows whose maximum is one of those."""
+    g = torch.Generator().manual_seed(17)
+    x = torch.randn(10, 6007, generator=g)
+    x[0] *= 300
+    x[1] *= 2.0 ** -18
+    x[2] = x[2].clamp(max=0)  # (the maximum is 0)
+    x[3] = -x[3].abs() - 2.0 ** -17
+    x[4] = 0
+    x[4, 100:200] = 2.0 ** -20 * torch.randn(100, generator=g)
+    x[5, ::3] *= 2.0 ** -17
+    x[6] -= 400
+    x[7, 11] = 256.0
+    x[8] = torch.where(x[8] > 0, 255.0, -257.0)
+    x[9, :5000] = -math.inf
+    x = x.to(torch.bfloat16)
+    u = torch.rand(10, generator=g)
+    for kw in ({}, dict(temperature=0.01), dict(temperature=30.0), dict(top_k=7), dict(top_k=3000), dict(top_p=0.4),
+               dict(top_p=0.999), dict(temperature=0.03, top_p=0.9), dict(top_k=2000, top_p=0.6, min_p=1e-3),
+               dict(temperature=200.0, top_p=0.7)):
+        _check(x, u, **kw)
