@@ -18,11 +18,17 @@
 // HBM, the later ones from the Infinity Cache):
 //   no filter       open, pick
 //   min-p alone     scan, mass, pick
+//   a small top-k   scan, list, draw
 //   top-k or top-p  bf16: count, cut, mass, pick
 //                   fp16, fp32: scan, hist, cut, mass, pick
-// (a setting that comes row by row may be any of its values)
+// (a setting that comes row by row may be any of its values; fp16's and
+// fp32's rows of a small top-k of their own go by a list between the others)
 //   open   the fp64 mass and the maximum of each run
 //   scan   max and log-sum-exp (fp32)
+//   list   the few logits at or above a bound on the k-th, taken from the scan's
+//          maxima, and (draw) the token from them, ordered. One reading of the
+//          row and two launches less than bins: 256 rows of 151936 fp32 logits
+//          with k = 50 take 65 us, 124 by bins; one bf16 row of 128256 20 us, 30.
 //   hist   counts, and for top-p masses, in bins linear in max - x
 //   count  counts in bins of one bf16 value each, which give the maximum, the
 //          sum and every mass
@@ -35,8 +41,8 @@
 //
 // What bounds it: the first pass of 256 rows of 151936 bf16 logits (78 MB) runs
 // at HBM's rate (scan 15 us); the bins' LDS atomics (count 23 us) and the mass
-// table's LDS gathers (mass 34 us, 33 cycles a wave's) are LDS-bound, cut and
-// pick (11 and 7 us) chains of latencies. 77 us in all with top-p, 34 without
+// table's LDS gathers (mass 34 us, 33 cycles a wave's) are LDS-bound, cut, draw
+// and pick (11, 7 and 7 us) chains of latencies. 77 us in all with top-p, 34 without
 // filters; few rows are bound by those chains, 4 to 14 us a launch.
 //
 // Masses are fp64: with 32-bit ones the running sums of a flat row of 1e5
@@ -68,6 +74,11 @@ constexpr double kRange = 24;
 constexpr double kTempMin = 0x1p-64, kTempMax = 0x1p64;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 constexpr int kGroups = 256;          // maxima that a bound on the k-th logit is taken from
+// Rows of few kept logits go by a list of those at or above that bound: for k = 208 of 256 groups it has about
+// 256 ln(256 / 48) = 430 of them, for k = 50 some 56.
+constexpr int kListMost = 208;        // k of such a row at most
+constexpr int kPartList = 512, kList = 768;  // room for a block's, and a row's
+__host__ __device__ constexpr int list_most(int runs) { return 4 * runs < kListMost ? 4 * runs : kListMost; }
 
 // A setting of every row, or one each.
 struct Setting {
@@ -120,6 +131,10 @@ struct Cut {
   uint32_t ties, equal;
   uint32_t count;  // logits kept
 };
+struct Listed {
+  float x;
+  int col;
+};
 struct SampleArgs {
   int64_t* ids;
   float* logp;
@@ -134,6 +149,7 @@ struct SampleArgs {
   int split;       // blocks of a row
   int open;        // no row has a filter
   int has_cuts;    // cuts is written
+  int lists;       // rows of few kept logits go by a list
   double magic;    // 2^(52 - b): e + magic holds e in b fixed-point bits
   // workspace
   float *part_max, *part_sum;  // [rows][split]
@@ -143,6 +159,8 @@ struct SampleArgs {
   float *run_max, *run_ref;    // of an open call: the run's maximum, and the logit whose mass its masses take as 1
   void* hist;                  // Hist<T> [rows][split], split > 1
   Cut* cuts;                   // [rows]
+  Listed* list;                // [rows][split][kPartList]
+  uint32_t* listed;            // [rows][split] how many (more than kPartList: not all are there)
 };
 
 __device__ __forceinline__ double setting(const Setting& s, int64_t row) { return s.rows ? s.rows[row] : s.all; }
@@ -152,7 +170,7 @@ struct Asked {
   double temp, top_p, min_p;
   double k;  // log2(e) / T
   int64_t top_k;
-  bool by_k, by_p;
+  bool by_k, by_p, by_list;
   bool in_range;
 };
 __device__ __forceinline__ Asked asked(const SampleArgs& g, int64_t row) {
@@ -168,6 +186,7 @@ __device__ __forceinline__ Asked asked(const SampleArgs& g, int64_t row) {
   a.k = kLog2eD / a.temp;
   a.by_k = a.top_k > 0 && a.top_k < g.cols;
   a.by_p = a.top_p < 1.0;
+  a.by_list = g.lists && a.by_k && a.top_k <= list_most(g.runs);
   a.in_range = a.temp >= kTempMin && a.temp <= kTempMax && u >= 0.f && u <= 1.f && a.top_p == a.top_p &&
                a.min_p == a.min_p;
   return a;
@@ -231,8 +250,8 @@ __device__ __forceinline__ Pack<T, 16 / sizeof(T)> load_cols(const T* row, int c
   return pack<T, VEC>(f);
 }
 
-// A row's runs first, first + waves, ...: look(pack) for each 16 bytes of a lane, done(run) after each run. A wave has
-// two packs on their way. The loop stays rolled: unrolled over a run (32 logits a lane) these kernels have 25 to 80 KB
+// A row's runs first, first + waves, ...: look(pack, column) for each 16 bytes of a lane, done(run) after each run. A
+// wave has two packs on their way. The loop stays rolled: unrolled over a run (32 logits a lane) these kernels have 25 to 80 KB
 // of code, and fetching it, not the logits, set their time (hist of 64 x 151936: 33 us; 24 rolled).
 template <typename T, typename L, typename D>
 __device__ __forceinline__ void each_run(const T* row, int cols, int run_cols, int runs, int first, int waves, L&& look,
@@ -257,7 +276,7 @@ __device__ __forceinline__ void each_run(const T* row, int cols, int run_cols, i
     const Pack<T, VEC> p = p0;
     p0 = p1;
     p1 = load();
-    look(p);
+    look(p, run * run_cols + at + lane_col);
     at += kStep;
     if (at == run_cols) {
       done(run);
@@ -347,6 +366,18 @@ __device__ __forceinline__ int first_or_last(bool passes, bool some, int* tmp) {
   return first < kLanes ? first : last;
 }
 
+// The smallest float x with e^((x - max) / T) >= min_p (-inf without min-p). log2 min_p: the instruction's, off by some
+// 2^-22, and what is left of min_p after it (2^-100 of the largest probability is as good as none).
+__device__ __forceinline__ float least_of_min_p(const Asked& a, float max) {
+  if (!(a.min_p > 0.0)) return -INFINITY;
+  if (a.min_p >= 1.0) return max;
+  const double p = fmax(a.min_p, 0x1p-100);
+  const double y = (double)log2_fast((float)p), rest = p * exp2_product(-y, 1.0) - 1.0;
+  const double least = (double)max + a.temp * kLn2D * (y + kLog2eD * (rest - 0.5 * rest * rest));
+  const float f = (float)least;
+  return (double)f < least ? nextafterf(f, INFINITY) : f;
+}
+
 // What the launches after the scan begin with, its loads in flight together: the row's settings, its maximum and sum of
 // e^(z - max) from its blocks' parts (every wave puts them together for itself), and its cut. ok: it has a distribution.
 struct Start {
@@ -366,16 +397,11 @@ struct Start {
     sum = wave_sum(m == -INFINITY ? s : s * exp2_fast((m - max) * (float)a.k));
     // (a NaN, a +inf or nothing above -inf leaves the sum NaN or 0)
     ok = a.in_range && sum > 0.f && sum < INFINITY && max < INFINITY;
-    if (with_cut && ok && a.min_p > 0.0) {
-      // e^((x - max) / T) >= min_p, as the smallest float that satisfies it. log2 min_p: the instruction's, off by some
-      // 2^-22, and what is left of min_p after it (2^-100 of the largest probability is as good as none).
-      const double p = fmax(fmin(a.min_p, 1.0), 0x1p-100);
-      const double y = (double)log2_fast((float)p), rest = p * exp2_product(-y, 1.0) - 1.0;
-      const double least = (double)max + a.temp * kLn2D * (y + kLog2eD * (rest - 0.5 * rest * rest));
-      float f = (float)(p < 1.0 ? least : (double)max);
-      if (p < 1.0 && (double)f < least) f = nextafterf(f, INFINITY);
-      if (f > cut.x) cut = {f, 0xffffffffu, 0, cut.count};
-    }
+    if (with_cut && ok) cut_min_p();
+  }
+  __device__ __forceinline__ void cut_min_p() {
+    const float f = least_of_min_p(a, max);
+    if (f > cut.x) cut = {f, 0xffffffffu, 0, cut.count};
   }
 };
 
@@ -448,7 +474,7 @@ __device__ __forceinline__ void scan_block(const T* x, const SampleArgs& g, int 
   float m = -INFINITY, z = 0.f, rm = -INFINITY;  // rm: of the run
   each_run(
       x, g.cols, g.run_cols, g.runs, part * kWaves + wave, split * kWaves,
-      [&](const Pack<T, VEC>& p) {
+      [&](const Pack<T, VEC>& p, int) {
         float v[VEC];
         unpack(p, v);
         float q = v[0];
@@ -491,7 +517,7 @@ __global__ __launch_bounds__(kLanes) void sample_scan_kernel(SampleArgs g) {
   const Asked a = asked(g, row);
   float max, sum;
   scan_block(static_cast<const T*>(g.logits) + row * g.ld, g, (int)(blockIdx.x % g.split), g.split, (float)a.k,
-             a.by_k ? g.quarters + row * g.runs * 4 : nullptr, sh, &max, &sum);
+             a.by_list ? g.quarters + row * g.runs * 4 : nullptr, sh, &max, &sum);
   if (threadIdx.x == 0) g.part_max[blockIdx.x] = max, g.part_sum[blockIdx.x] = sum;
 }
 
@@ -516,7 +542,7 @@ __global__ __launch_bounds__(kLanes) void sample_open_kernel(SampleArgs g) {
   // m: this lane's maximum in the run, and (without the table) the logit whose mass is 1
   float m = -INFINITY;
   double mass = 0.0;
-  auto by_polynomial = [&](const Pack<T, VEC>& p) {
+  auto by_polynomial = [&](const Pack<T, VEC>& p, int) {
     float v[VEC], n = m;
     unpack(p, v);
 #pragma unroll
@@ -545,7 +571,7 @@ __global__ __launch_bounds__(kLanes) void sample_open_kernel(SampleArgs g) {
     if (use_table) {
       each_run(
           x, g.cols, g.run_cols, g.runs, first, waves,
-          [&](const Pack<T, VEC>& p) {
+          [&](const Pack<T, VEC>& p, int) {
             float v[VEC];
             unpack(p, v);
 #pragma unroll
@@ -672,9 +698,8 @@ struct Row {
     }
   }
 
-  // Adds the runs of one block (part of split) to h; logits below `least` are left out (bf16: none is, and masses are
-  // those of the bins of several).
-  __device__ __forceinline__ void fill(Hist<T>& h, int part, int split, float least, bool masses) const {
+  // Fills h with the runs of one block (part of split); bf16's masses are those of the bins of several.
+  __device__ __forceinline__ void fill(Hist<T>& h, int part, int split, bool masses) const {
     for (int i = threadIdx.x; i < B::kCount; i += kLanes) h.count[i] = 0;
     for (int i = threadIdx.x; i < B::kMasses; i += kLanes) h.mass[i] = 0;
     __syncthreads();
@@ -685,7 +710,7 @@ struct Row {
       constexpr int kLow = Bins<__bf16>::kUsed - 1;
       each_run(
           x, cols, run_cols, runs, first, waves,
-          [&](const Pack<T, VEC>& p) {
+          [&](const Pack<T, VEC>& p, int) {
             typename B::Two low2 = (typename B::Two)((short)B::kSide), high2 = (typename B::Two)((short)0);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -708,13 +733,9 @@ struct Row {
       constexpr int kLow = B::kCount - 1;
       each_run(
           x, cols, run_cols, runs, first, waves,
-          [&](const Pack<T, VEC>& p) {
+          [&](const Pack<T, VEC>& p, int) {
             float v[VEC];
             unpack(p, v);
-            float most = v[0];
-#pragma unroll
-            for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
-            if (!__any(most >= least)) return;
             u64 e[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) e[i] = 0;
@@ -725,11 +746,11 @@ struct Row {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
               const int b = bin_of(v[i]);
-              if (v[i] >= least && b < kLow) {
+              if (b < kLow) {
                 atomicAdd(&h.count[b], 1u);
                 if (masses) atomicAdd(&h.mass[b], e[i]);
               } else {
-                ++low;  // (what is left out counts as low: the k-th logit lies above)
+                ++low;
                 low_mass += e[i];
               }
             }
@@ -876,13 +897,220 @@ struct Row {
   }
 };
 
-// A lower bound of the k-th largest logit, k <= kGroups: the k-th largest of the maxima of kGroups disjoint sets of
-// columns (each of those k is a logit of its own), put together from the scan's. Its value is the largest that k of them
-// reach; four threads count for each.
+// ---- mass -------------------------------------------------------------------
+template <typename T> struct MassShared {
+  double table[Bins<T>::kExact ? Bins<__bf16>::kUsed : 1];
+};
+// The kept masses of one block's runs (part of split).
+template <typename T>
+__device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int part, int split, const Start& st,
+                                           MassShared<T>& sh) {
+  constexpr int VEC = 16 / sizeof(T);
+  constexpr bool kTable = Bins<T>::kExact;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const Row<T> r(g, row, st.a, st.max);
+  const Cut cut = st.cut;
+  const bool all_ties = cut.ties >= cut.equal;
+  auto kept = [&](float v) { return all_ties ? v >= cut.x : v > cut.x; };
+  double mass = 0.0;
+  uint32_t ties = 0;  // (the wave's)
+  const int first = part * kWaves + wave, waves = split * kWaves;
+  auto count_ties = [&](const Pack<T, VEC>& p) {
+    if (all_ties) return;
+    float v[VEC];
+    unpack(p, v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) ties += __popcll(__ballot(v[i] == cut.x));
+  };
+  auto done = [&](int run) {
+    mass = wave_total(mass);
+    if (lane == 0) g.run_mass[row * g.runs + run] = mass, g.run_ties[row * g.runs + run] = ties;
+    mass = 0.0;
+    ties = 0;
+  };
+  if constexpr (kTable) {
+    // few are kept: the table costs more than their polynomials (2 us; 1 in 64 of 38000 logits a block 0.6)
+    if (cut.count > (uint32_t)g.cols / 64) {
+      const int reach = Bins<T>::of(cut.x);
+      fill_table(sh.table, reach, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
+      each_run(
+          r.x, g.cols, g.run_cols, g.runs, first, waves,
+          [&](const Pack<T, VEC>& p, int) {
+            mass += sum_table(sh.table, p, reach, [&](float y) { return kept(y) ? r.mass(y) : 0.0; });
+            count_ties(p);
+          },
+          done);
+      return;
+    }
+  }
+  each_run(
+      r.x, g.cols, g.run_cols, g.runs, first, waves,
+      [&](const Pack<T, VEC>& p, int) {
+        float v[VEC];
+        unpack(p, v);
+        float most = v[0];
+#pragma unroll
+        for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
+        if (__any(most >= cut.x)) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) mass += kept(v[i]) ? r.mass(v[i]) : 0.0;
+          count_ties(p);
+        }
+      },
+      done);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
+  __shared__ MassShared<T> sh;
+  const int64_t row = blockIdx.x / g.split;
+  const Start st(g, row, true);
+  if (st.ok && !st.a.by_list) mass_block<T>(g, row, (int)(blockIdx.x % g.split), g.split, st, sh);
+}
+
+// ---- pick -------------------------------------------------------------------
+struct PickShared {
+  double dtmp[kWaves], base;
+  uint32_t utmp[kWaves], ties;
+  float ftmp[kWaves];
+  int itmp[2 * kWaves], run;
+};
+// The row's token from the masses of its runs; `start` gives its Start.
+template <typename T, typename S>
+__device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& start, PickShared& sh) {
+  constexpr int kCols = 2;  // columns a thread, in order: runs of up to 2048
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const double* run_mass = g.run_mass + row * g.runs;
+  const uint32_t* run_ties = g.run_ties + row * g.runs;
+  const float *run_max = g.run_max + row * g.runs, *run_ref = g.run_ref + row * g.runs;
+  const int per = (g.runs + kLanes - 1) / kLanes;  // runs a thread, in order
+  const int r0 = min(g.runs, (int)threadIdx.x * per), r1 = min(g.runs, r0 + per);
+  // the first run's records, on the way while the row's start is put together (mostly there is no other)
+  const int any_run = min(r0, g.runs - 1);
+  const double mass0 = run_mass[any_run];
+  const uint32_t ties0 = run_ties[any_run];
+  const float max0 = run_max[any_run], ref0 = run_ref[any_run];
+  Start st = start();
+  const Asked& a = st.a;
+  const float u = g.u[row];
+
+  bool fine = a.in_range;
+  if (g.open) {
+    float m = -INFINITY;
+    for (int i = r0; i < r1; ++i) m = fmaxf(m, i == r0 ? max0 : run_max[i]);
+    m = wave_max(m);
+    if (lane == 0) sh.ftmp[wave] = m;
+    __syncthreads();
+    st.max = sh.ftmp[0];
+    for (int i = 1; i < kWaves; ++i) st.max = fmaxf(st.max, sh.ftmp[i]);
+  } else {
+    fine = st.ok;
+  }
+  if (!fine) {
+    if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
+    return;
+  }
+  const float max = st.max;
+  const Row<T> r(g, row, st.a, st.max);
+  const Cut cut = g.open ? Cut{-INFINITY, 0xffffffffu, 0, 0} : st.cut;
+  const bool all_ties = cut.ties >= cut.equal;
+  const double each = all_ties ? 0.0 : r.mass(cut.x);
+
+  // the masses of the runs (an open row's in terms of their own reference)
+  uint32_t ties = 0, seen = 0;
+  if (!all_ties) {
+    for (int i = r0; i < r1; ++i) ties += i == r0 ? ties0 : run_ties[i];
+    uint32_t all;
+    seen = block_before<uint32_t>(ties, sh.utmp, &all);
+  }
+  auto mass_of = [&](int i, uint32_t& ties_before) {
+    const double m = i == r0 ? mass0 : run_mass[i];
+    if (g.open) return m * exp2_product((double)(i == r0 ? ref0 : run_ref[i]) - (double)max, r.k);
+    if (all_ties) return m;
+    const uint32_t t = i == r0 ? ties0 : run_ties[i], left = cut.ties - min(cut.ties, ties_before);
+    ties_before += t;
+    return m + each * (double)min(left, t);
+  };
+  double mass = 0.0;
+  uint32_t rank = seen;
+#pragma unroll 1
+  for (int i = r0; i < r1; ++i) mass += mass_of(i, rank);
+  double total;
+  const double before = block_before<double>(mass, sh.dtmp, &total);
+  if (!(total > 0.0 && total < INFINITY && max < INFINITY)) {  // (only an open row's can be)
+    if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
+    return;
+  }
+  const double target = (double)u * total;
+  // the first thread that passes the target; if none does, the last one with any mass
+  if ((int)threadIdx.x == first_or_last(mass > 0.0 && before + mass > target, mass > 0.0, sh.itmp)) {
+    double s = before;
+    int run = r0;
+    rank = seen;
+#pragma unroll 1
+    for (int i = r0; i < r1; ++i) {
+      const uint32_t rank_before = rank;
+      const double m = mass_of(i, rank);
+      if (m > 0.0) run = i, sh.base = s, sh.ties = rank_before;
+      s += m;
+      if (m > 0.0 && s > target) break;
+    }
+    sh.run = run;
+  }
+  __syncthreads();
+  const int c0 = sh.run * g.run_cols + (int)threadIdx.x * kCols, c1 = min(g.cols, (sh.run + 1) * g.run_cols);
+  float v[kCols];
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) v[i] = c0 + i < c1 ? to_f32<T>(r.x[c0 + i]) : -INFINITY;
+  rank = sh.ties;
+  const double base = sh.base;
+  if (!all_ties) {
+    ties = 0;
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) ties += v[i] == cut.x ? 1 : 0;
+    uint32_t all;
+    rank += block_before<uint32_t>(ties, sh.utmp, &all);
+  }
+  double e[kCols];
+  mass = 0.0;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    bool keep = v[i] >= cut.x;
+    if (!all_ties && v[i] == cut.x) keep = rank++ < cut.ties;
+    e[i] = keep ? r.mass(v[i]) : 0.0;
+    mass += e[i];
+  }
+  double run_total;
+  double s = base + block_before<double>(mass, sh.dtmp, &run_total);
+  if ((int)threadIdx.x != first_or_last(mass > 0.0 && s + mass > target, mass > 0.0, sh.itmp)) return;
+  int id = -1;
+  float at = 0.f;
+  bool done = false;
+#pragma unroll
+  for (int i = 0; i < kCols; ++i) {
+    if (!done && e[i] > 0.0) id = c0 + i, at = v[i];
+    s += e[i];
+    done = done || (e[i] > 0.0 && s > target);
+  }
+  g.ids[row] = id;
+  g.logp[row] = (float)(((double)at - (double)max) * r.k * kLn2D) - log_fast(g.open ? (float)total : st.sum);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
+  __shared__ PickShared sh;
+  const int64_t row = blockIdx.x;
+  if (g.lists && asked(g, row).by_list) return;
+  pick_row<T>(g, row, [&] { return Start(g, row, true); }, sh);
+}
+
+// ---- list -------------------------------------------------------------------
+// A lower bound of the k-th largest logit: the k-th largest of the maxima of kGroups disjoint sets of columns (each of
+// those k is a logit of its own), put together from the scan's. Its value is the largest that k of them reach; four
+// threads count for each.
 __device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row, const Asked& a, BoundShared& sh) {
-  static_assert(kLanes == 4 * kGroups, "four threads a group");
+  static_assert(kLanes == 4 * kGroups && kListMost <= kGroups, "four threads a group");
   const int n = 4 * g.runs, i = threadIdx.x % kGroups, part = threadIdx.x / kGroups;
-  if (!a.by_k || a.top_k > min(n, kGroups)) return -INFINITY;
   if (part == 0) {
     float m = -INFINITY;
 #pragma unroll 1
@@ -908,18 +1136,216 @@ __device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row
   return best;
 }
 
-// WHOLE: one block has the whole row (split 1) and goes on to the cut.
-template <typename T, bool WHOLE>
-__global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
-  __shared__ __align__(16) typename std::conditional<WHOLE, CutShared<T>, HistShared<T>>::type sh;
+// Lists the logits of one block's runs that reach `least` (all finite ones if that is -inf), in any order.
+struct ListShared {
+  uint32_t n;
+  Listed list[kPartList];
+};
+template <typename T>
+__device__ __forceinline__ void list_block(const T* x, const SampleArgs& g, int64_t row, int part, float least,
+                                           ListShared& sh) {
+  constexpr int VEC = 16 / sizeof(T);
+  const float bound = fmaxf(least, -3.402823466e38f);
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  each_run(
+      x, g.cols, g.run_cols, g.runs, part * kWaves + (int)threadIdx.x / kWave, g.split * kWaves,
+      [&](const Pack<T, VEC>& p, int c) {
+        float v[VEC];
+        unpack(p, v);
+        float most = v[0];
+#pragma unroll
+        for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
+        if (!__any(most >= bound)) return;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          if (v[i] >= bound) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < (uint32_t)kPartList) sh.list[at] = {v[i], c + i};
+          }
+        }
+      },
+      [](int) {});
+  __syncthreads();
+  const int64_t block = row * g.split + part;
+  for (int i = threadIdx.x; i < (int)min(sh.n, (uint32_t)kPartList); i += kLanes) g.list[block * kPartList + i] = sh.list[i];
+  if (threadIdx.x == 0) g.listed[block] = sh.n;
+}
+
+// Draws a row's token from its list; false if that has not room for all.
+struct DrawShared {
+  u64 key[kList];       // of the listed: larger x, then lower column, first
+  uint32_t rank[kList];
+  float x[kList];       // in that order
+  int col[kList];
+  double e[kListMost];  // of the kept, by column
+  int from[kListMost];
+  double dtmp[kWaves];
+  int itmp[2 * kWaves];
+};
+__device__ __forceinline__ bool draw_listed(const SampleArgs& g, int64_t row, const Start& st, DrawShared& sh) {
+  const Asked& a = st.a;
+  const int lane = threadIdx.x % kWave, t = threadIdx.x;
+  const float u = g.u[row];
+  const uint32_t in_part = lane < g.split ? g.listed[row * g.split + lane] : 0;
+  const uint32_t incl = wave_scan(in_part), n = of_lane63(incl);
+  if (__any(in_part > (uint32_t)kPartList) || n > (uint32_t)kList) return false;
+  int part = 0;
+  uint32_t before_part = 0;
+#pragma unroll 1
+  for (int i = 0; i < g.split - 1; ++i) {
+    const uint32_t upto = of_lane(incl, i);
+    if ((uint32_t)t >= upto) part = i + 1, before_part = upto;
+  }
+  Listed mine = {0.f, 0};
+  if (t < (int)n) {
+    mine = g.list[(row * g.split + part) * kPartList + (t - before_part)];
+    sh.key[t] = (u64)key_of<float>(mine.x) << 32 | (uint32_t)~mine.col;
+    sh.rank[t] = 0;
+  }
+  if (t < kListMost) sh.e[t] = 0.0;
+  __syncthreads();
+  // the rank of each, by comparison with all; the threads share them out
+  {
+    int width = kWave;
+    while (width < (int)n) width *= 2;
+    const int i = t & (width - 1), q = t / width, each = ((int)n + kLanes / width - 1) / (kLanes / width);
+    if (i < (int)n) {
+      const u64 key = sh.key[i];
+      uint32_t rank = 0;
+#pragma unroll 4
+      for (int j = q * each; j < min((int)n, (q + 1) * each); ++j) rank += sh.key[j] > key ? 1 : 0;
+      if (rank) atomicAdd(&sh.rank[i], rank);
+    }
+  }
+  __syncthreads();
+  if (t < (int)n) {
+    const uint32_t r = sh.rank[t];
+    sh.x[r] = mine.x;
+    sh.col[r] = mine.col;
+  }
+  __syncthreads();
+  // the filters keep a prefix of that order
+  const int k = min((int)a.top_k, (int)n);
+  const float x = t < k ? sh.x[t] : -INFINITY;
+  const int col = t < k ? sh.col[t] : 0x7fffffff;
+  const double e = exp2_product((double)x - (double)st.max, a.k);
+  double total;
+  const double above = block_before<double>(e, sh.dtmp, &total);
+  const bool keep = t < k && (!a.by_p || t == 0 || above < a.top_p * total) && x >= least_of_min_p(a, st.max);
+  __syncthreads();
+  if (t < k) sh.col[t] = keep ? col : 0x7fffffff;
+  __syncthreads();
+  if (keep) {
+    int at = 0;
+#pragma unroll 4
+    for (int j = 0; j < k; ++j) at += sh.col[j] < col ? 1 : 0;
+    sh.e[at] = e;
+    sh.from[at] = t;
+  }
+  __syncthreads();
+  const double mass = t < kListMost ? sh.e[t] : 0.0;
+  const double s = block_before<double>(mass, sh.dtmp, &total);
+  if (t == first_or_last(mass > 0.0 && s + mass > (double)u * total, mass > 0.0, sh.itmp)) {
+    const int r = sh.from[t];
+    g.ids[row] = sh.col[r];
+    g.logp[row] = (float)(((double)sh.x[r] - (double)st.max) * a.k * kLn2D) - log_fast(st.sum);
+  }
+  if (t == 0) g.cuts[row].count = 0;
+  return true;
+}
+
+// What a row that goes by a list may need: the list is short of room if many logits equal the bound, and then one block
+// goes the way of the others (cut, mass, pick) for the row (160 us for 64 rows of 151936 equal bf16 logits; rows with 512
+// logits equal to the k-th are none that a model gives).
+template <typename T>
+union __align__(16) ListedShared {
+  ListShared list;
+  DrawShared draw;
+  CutShared<T> cut;
+  struct {
+    MassShared<T> mass;
+    PickShared pick;
+  } rest;
+  __device__ ListedShared() {}
+};
+template <typename T>
+__device__ __forceinline__ void end_listed(const SampleArgs& g, int64_t row, Start& st, ListedShared<T>& sh) {
+  if (draw_listed(g, row, st, sh.draw)) return;
+  const Row<T> r(g, row, st.a, st.max);
+  r.fill(sh.cut.hist, 0, 1, st.a.by_p);
+  st.cut = r.find(sh.cut, st.a);
+  st.cut_min_p();
+  __syncthreads();
+  mass_block<T>(g, row, 0, 1, st, sh.rest.mass);
+  __syncthreads();
+  pick_row<T>(g, row, [&] { return st; }, sh.rest.pick);
+}
+
+// A call whose rows all go by lists.
+template <typename T>
+__global__ __launch_bounds__(kLanes) void sample_list_kernel(SampleArgs g) {
   __shared__ BoundShared bound;
+  __shared__ ListShared sh;
   const int64_t row = blockIdx.x / g.split;
   const Start st(g, row, false);
+  if (!st.ok) return;
+  list_block(static_cast<const T*>(g.logits) + row * g.ld, g, row, (int)(blockIdx.x % g.split),
+             least_of_top_k(g, row, st.a, bound), sh);
+}
+template <typename T>
+__global__ __launch_bounds__(kLanes) void sample_draw_kernel(SampleArgs g) {
+  __shared__ ListedShared<T> sh;
+  const int64_t row = blockIdx.x;
+  Start st(g, row, false);
+  if (st.ok) {
+    end_listed(g, row, st, sh);
+  } else if (threadIdx.x == 0) {
+    g.ids[row] = -1;
+    g.logp[row] = __builtin_nanf("");
+  }
+}
+
+// ---- hist, cut ----------------------------------------------------------------
+template <typename T, bool MIXED>
+union __align__(16) RowShared {
+  CutShared<T> cut;
+  typename std::conditional<MIXED, ListedShared<T>, char>::type listed;
+  __device__ RowShared() {}
+};
+template <typename T, bool MIXED>
+union __align__(16) PartShared {
+  HistShared<T> cut;
+  typename std::conditional<MIXED, ListShared, char>::type listed;
+  __device__ PartShared() {}
+};
+// WHOLE: one block has the whole row (split 1) and goes on to the cut. MIXED: rows may go by lists.
+template <typename T, bool WHOLE, bool MIXED>
+__global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
+  __shared__ typename std::conditional<WHOLE, RowShared<T, MIXED>, PartShared<T, MIXED>>::type sh;
+  const int64_t row = blockIdx.x / g.split;
+  const int part = (int)(blockIdx.x % g.split);
+  Start st(g, row, false);
+  if (MIXED && WHOLE && !st.ok && st.a.by_list && threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
   if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
   const Row<T> r(g, row, st.a, st.max);
-  r.fill(sh.hist, (int)(blockIdx.x % g.split), g.split, least_of_top_k(g, row, st.a, bound), st.a.by_p);
+  if constexpr (MIXED) {
+    __shared__ BoundShared bound;
+    if (st.a.by_list) {
+      const float least = least_of_top_k(g, row, st.a, bound);
+      if constexpr (WHOLE) {
+        list_block(r.x, g, row, part, least, sh.listed.list);
+        __syncthreads();
+        end_listed(g, row, st, sh.listed);
+      } else {
+        list_block(r.x, g, row, part, least, sh.listed);
+      }
+      return;
+    }
+  }
+  r.fill(sh.cut.hist, part, g.split, st.a.by_p);
   if constexpr (WHOLE) {
-    const Cut cut = r.find(sh, st.a);
+    const Cut cut = r.find(sh.cut, st.a);
     if (threadIdx.x == 0) g.cuts[row] = cut;
   } else {
     __syncthreads();
@@ -928,7 +1354,7 @@ __global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
     // (masses first; they are not read without top-p)
     const int skip = st.a.by_p ? 0 : (int)(sizeof(u64) * Bins<T>::kMasses / 16);
     for (int i = skip + (int)threadIdx.x; i < (int)(sizeof(Hist<T>) / 16); i += kLanes)
-      reinterpret_cast<u32x4*>(&to)[i] = reinterpret_cast<const u32x4*>(&sh.hist)[i];
+      reinterpret_cast<u32x4*>(&to)[i] = reinterpret_cast<const u32x4*>(&sh.cut.hist)[i];
   }
 }
 
@@ -946,13 +1372,21 @@ __device__ __forceinline__ V sum_parts(const char* p, size_t stride, int split) 
 }
 
 // (split > 1)
-template <typename T>
+template <typename T, bool MIXED>
 __global__ __launch_bounds__(kLanes) void sample_cut_kernel(SampleArgs g) {
   typedef u64 u64x2 __attribute__((ext_vector_type(2)));
-  __shared__ __align__(16) CutShared<T> sh;
+  __shared__ RowShared<T, MIXED> all;
   const int64_t row = blockIdx.x;
-  const Start st(g, row, false);
+  Start st(g, row, false);
+  if (MIXED && !st.ok && st.a.by_list && threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
   if (!st.ok || (!st.a.by_k && !st.a.by_p)) return;
+  if constexpr (MIXED) {
+    if (st.a.by_list) {
+      end_listed(g, row, st, all.listed);
+      return;
+    }
+  }
+  CutShared<T>& sh = all.cut;
   const Row<T> r(g, row, st.a, st.max);
   const Hist<T>* from = static_cast<const Hist<T>*>(g.hist) + row * g.split;
 #pragma unroll 1
@@ -974,7 +1408,7 @@ __global__ __launch_bounds__(kLanes) void sample_cut_kernel(SampleArgs g) {
 // scan and hist in one block.
 constexpr double kTinyTemp = 0x1p-4;
 constexpr int kFlag = 3;  // the place of h.mass that counts what was flagged
-struct CountShared : CutShared<__bf16> {
+struct CountShared {
   ScanShared scan;
   int first[kWaves];
 };
@@ -989,7 +1423,7 @@ __device__ __forceinline__ void count_block(Hist<__bf16>& h, const SampleArgs& g
   uint32_t low = 0;
   each_run(
       x, g.cols, g.run_cols, g.runs, part * kWaves + (int)threadIdx.x / kWave, g.split * kWaves,
-      [&](const Pack<__bf16, 8>& p) {
+      [&](const Pack<__bf16, 8>& p, int) {
         B::Two least = (B::Two)((short)B::kSide), most = (B::Two)((short)0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1016,7 +1450,8 @@ __device__ __forceinline__ void count_block(Hist<__bf16>& h, const SampleArgs& g
 }
 
 // The row's maximum, sum and cut from the counts of all its columns.
-__device__ __forceinline__ void cut_counted(CountShared& sh, const SampleArgs& g, int64_t row, const Asked& a) {
+__device__ __forceinline__ void cut_counted(CutShared<__bf16>& sh, CountShared& own, const SampleArgs& g, int64_t row,
+                                            const Asked& a) {
   typedef Bins<__bf16> B;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const __bf16* x = static_cast<const __bf16*>(g.logits) + row * g.ld;
@@ -1028,19 +1463,19 @@ __device__ __forceinline__ void cut_counted(CountShared& sh, const SampleArgs& g
   for (int i = kEach - 1; i >= 0; --i)
     if (sh.hist.count[kEach * threadIdx.x + i]) first = kEach * threadIdx.x + i;
   const u64 some = __ballot(first < B::kCount);
-  if (lane == 0) sh.first[wave] = B::kCount;
-  if (some && lane == __builtin_ctzll(some)) sh.first[wave] = first;
+  if (lane == 0) own.first[wave] = B::kCount;
+  if (some && lane == __builtin_ctzll(some)) own.first[wave] = first;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) first = min(first, sh.first[i]);
+  for (int i = 0; i < kWaves; ++i) first = min(first, own.first[i]);
   float max = B::value(first), sum = 0.f;
   Cut cut = {-INFINITY, 0xffffffffu, 0, 0xffffffffu};
   const bool cuts = a.by_k || a.by_p, again = sh.hist.mass[kFlag] || B::several(first);
-  if (again) scan_block(x, g, 0, 1, (float)a.k, nullptr, sh.scan, &max, &sum);
+  if (again) scan_block(x, g, 0, 1, (float)a.k, nullptr, own.scan, &max, &sum);
   const Row<__bf16> r(g, row, a, max);
   const bool ok = !again || (sum > 0.f && sum < INFINITY && max < INFINITY);
   __syncthreads();
-  if (again && ok && cuts) r.fill(sh.hist, 0, 1, -INFINITY, a.by_p);
+  if (again && ok && cuts) r.fill(sh.hist, 0, 1, a.by_p);
   if (!again && threadIdx.x == 0)  // in terms of the maximum from here on
     sh.hist.mass[1] = (u64)((double)sh.hist.mass[1] * exp2_product(-(double)max, a.k) + 0.5);
   if (ok && (cuts || !again)) {
@@ -1058,12 +1493,15 @@ __device__ __forceinline__ void cut_counted(CountShared& sh, const SampleArgs& g
 
 template <bool WHOLE>
 __global__ __launch_bounds__(kLanes) void sample_count_kernel(SampleArgs g) {
-  __shared__ __align__(16) typename std::conditional<WHOLE, CountShared, HistShared<__bf16>>::type sh;
+  __shared__ __align__(16) typename std::conditional<WHOLE, CutShared<__bf16>, HistShared<__bf16>>::type sh;
+  __shared__ CountShared own;
   const int64_t row = blockIdx.x / g.split;
+  const int part = (int)(blockIdx.x % g.split);
   const Asked a = asked(g, row);
-  count_block(sh.hist, g, static_cast<const __bf16*>(g.logits) + row * g.ld, a, (int)(blockIdx.x % g.split));
+  const __bf16* x = static_cast<const __bf16*>(g.logits) + row * g.ld;
+  count_block(sh.hist, g, x, a, part);
   if constexpr (WHOLE) {
-    cut_counted(sh, g, row, a);
+    cut_counted(sh, own, g, row, a);
   } else {
     __syncthreads();
     u32x4* to = reinterpret_cast<u32x4*>(static_cast<Hist<__bf16>*>(g.hist) + blockIdx.x);
@@ -1075,7 +1513,8 @@ __global__ __launch_bounds__(kLanes) void sample_count_kernel(SampleArgs g) {
 // (split > 1)
 __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) {
   typedef Bins<__bf16> B;
-  __shared__ __align__(16) CountShared sh;
+  __shared__ __align__(16) CutShared<__bf16> sh;
+  __shared__ CountShared own;
   const int64_t row = blockIdx.x;
   const Hist<__bf16>* from = static_cast<const Hist<__bf16>*>(g.hist) + row * g.split;
   const Asked a = asked(g, row);
@@ -1085,198 +1524,7 @@ __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) 
         sum_parts<u32x4>((const char*)&from->count[i], sizeof(Hist<__bf16>), g.split);
   if (threadIdx.x < B::kMasses) sh.hist.mass[threadIdx.x] =
       sum_parts<u64>((const char*)&from->mass[threadIdx.x], sizeof(Hist<__bf16>), g.split);
-  cut_counted(sh, g, row, a);
-}
-
-// ---- mass -------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
-  constexpr int VEC = 16 / sizeof(T);
-  constexpr bool kTable = Bins<T>::kExact;
-  __shared__ double table[kTable ? Bins<__bf16>::kUsed : 1];
-  const int64_t row = blockIdx.x / g.split;
-  const int part = blockIdx.x % g.split;
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const Start st(g, row, true);
-  if (!st.ok) return;
-  const Row<T> r(g, row, st.a, st.max);
-  const Cut cut = st.cut;
-  const bool all_ties = cut.ties >= cut.equal;
-  auto kept = [&](float v) { return all_ties ? v >= cut.x : v > cut.x; };
-  double mass = 0.0;
-  uint32_t ties = 0;  // (the wave's)
-  const int first = part * kWaves + wave, waves = g.split * kWaves;
-  auto count_ties = [&](const Pack<T, VEC>& p) {
-    if (all_ties) return;
-    float v[VEC];
-    unpack(p, v);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) ties += __popcll(__ballot(v[i] == cut.x));
-  };
-  auto done = [&](int run) {
-    mass = wave_total(mass);
-    if (lane == 0) g.run_mass[row * g.runs + run] = mass, g.run_ties[row * g.runs + run] = ties;
-    mass = 0.0;
-    ties = 0;
-  };
-  if constexpr (kTable) {
-    // few are kept: the table costs more than their polynomials (2 us; 1 in 64 of 38000 logits a block 0.6)
-    if (cut.count > (uint32_t)g.cols / 64) {
-      const int reach = Bins<T>::of(cut.x);
-      fill_table(table, reach, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
-      each_run(
-          r.x, g.cols, g.run_cols, g.runs, first, waves,
-          [&](const Pack<T, VEC>& p) {
-            mass += sum_table(table, p, reach, [&](float y) { return kept(y) ? r.mass(y) : 0.0; });
-            count_ties(p);
-          },
-          done);
-      return;
-    }
-  }
-  each_run(
-      r.x, g.cols, g.run_cols, g.runs, first, waves,
-      [&](const Pack<T, VEC>& p) {
-        float v[VEC];
-        unpack(p, v);
-        float most = v[0];
-#pragma unroll
-        for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
-        if (__any(most >= cut.x)) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) mass += kept(v[i]) ? r.mass(v[i]) : 0.0;
-          count_ties(p);
-        }
-      },
-      done);
-}
-
-// ---- pick -------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
-  constexpr int kCols = 2;  // columns a thread, in order: runs of up to 2048
-  __shared__ double dtmp[kWaves];
-  __shared__ uint32_t utmp[kWaves];
-  __shared__ float ftmp[kWaves];
-  __shared__ int itmp[2 * kWaves], sh_run;
-  __shared__ double sh_base;
-  __shared__ uint32_t sh_ties;
-  const int64_t row = blockIdx.x;
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const double* run_mass = g.run_mass + row * g.runs;
-  const uint32_t* run_ties = g.run_ties + row * g.runs;
-  const float *run_max = g.run_max + row * g.runs, *run_ref = g.run_ref + row * g.runs;
-  const int per = (g.runs + kLanes - 1) / kLanes;  // runs a thread, in order
-  const int r0 = min(g.runs, (int)threadIdx.x * per), r1 = min(g.runs, r0 + per);
-  // the first run's records, on the way while the row's start is put together (mostly there is no other)
-  const int any_run = min(r0, g.runs - 1);
-  const double mass0 = run_mass[any_run];
-  const uint32_t ties0 = run_ties[any_run];
-  const float max0 = run_max[any_run], ref0 = run_ref[any_run];
-  Start st(g, row, true);
-  const Asked& a = st.a;
-  const float u = g.u[row];
-
-  bool fine = a.in_range;
-  if (g.open) {
-    float m = -INFINITY;
-    for (int i = r0; i < r1; ++i) m = fmaxf(m, i == r0 ? max0 : run_max[i]);
-    m = wave_max(m);
-    if (lane == 0) ftmp[wave] = m;
-    __syncthreads();
-    st.max = ftmp[0];
-    for (int i = 1; i < kWaves; ++i) st.max = fmaxf(st.max, ftmp[i]);
-  } else {
-    fine = st.ok;
-  }
-  if (!fine) {
-    if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
-    return;
-  }
-  const float max = st.max;
-  const Row<T> r(g, row, st.a, st.max);
-  const Cut cut = g.open ? Cut{-INFINITY, 0xffffffffu, 0, 0} : st.cut;
-  const bool all_ties = cut.ties >= cut.equal;
-  const double each = all_ties ? 0.0 : r.mass(cut.x);
-
-  // the masses of the runs (an open row's in terms of their own reference)
-  uint32_t ties = 0, seen = 0;
-  if (!all_ties) {
-    for (int i = r0; i < r1; ++i) ties += i == r0 ? ties0 : run_ties[i];
-    uint32_t all;
-    seen = block_before<uint32_t>(ties, utmp, &all);
-  }
-  auto mass_of = [&](int i, uint32_t& ties_before) {
-    const double m = i == r0 ? mass0 : run_mass[i];
-    if (g.open) return m * exp2_product((double)(i == r0 ? ref0 : run_ref[i]) - (double)max, r.k);
-    if (all_ties) return m;
-    const uint32_t t = i == r0 ? ties0 : run_ties[i], left = cut.ties - min(cut.ties, ties_before);
-    ties_before += t;
-    return m + each * (double)min(left, t);
-  };
-  double mass = 0.0;
-  uint32_t rank = seen;
-#pragma unroll 1
-  for (int i = r0; i < r1; ++i) mass += mass_of(i, rank);
-  double total;
-  const double before = block_before<double>(mass, dtmp, &total);
-  if (!(total > 0.0 && total < INFINITY && max < INFINITY)) {  // (only an open row's can be)
-    if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
-    return;
-  }
-  const double target = (double)u * total;
-  // the first thread that passes the target; if none does, the last one with any mass
-  if ((int)threadIdx.x == first_or_last(mass > 0.0 && before + mass > target, mass > 0.0, itmp)) {
-    double s = before;
-    int run = r0;
-    rank = seen;
-#pragma unroll 1
-    for (int i = r0; i < r1; ++i) {
-      const uint32_t rank_before = rank;
-      const double m = mass_of(i, rank);
-      if (m > 0.0) run = i, sh_base = s, sh_ties = rank_before;
-      s += m;
-      if (m > 0.0 && s > target) break;
-    }
-    sh_run = run;
-  }
-  __syncthreads();
-  const int c0 = sh_run * g.run_cols + (int)threadIdx.x * kCols, c1 = min(g.cols, (sh_run + 1) * g.run_cols);
-  float v[kCols];
-#pragma unroll
-  for (int i = 0; i < kCols; ++i) v[i] = c0 + i < c1 ? to_f32<T>(r.x[c0 + i]) : -INFINITY;
-  rank = sh_ties;
-  const double base = sh_base;
-  if (!all_ties) {
-    ties = 0;
-#pragma unroll
-    for (int i = 0; i < kCols; ++i) ties += v[i] == cut.x ? 1 : 0;
-    uint32_t all;
-    rank += block_before<uint32_t>(ties, utmp, &all);
-  }
-  double e[kCols];
-  mass = 0.0;
-#pragma unroll
-  for (int i = 0; i < kCols; ++i) {
-    bool keep = v[i] >= cut.x;
-    if (!all_ties && v[i] == cut.x) keep = rank++ < cut.ties;
-    e[i] = keep ? r.mass(v[i]) : 0.0;
-    mass += e[i];
-  }
-  double run_total;
-  double s = base + block_before<double>(mass, dtmp, &run_total);
-  if ((int)threadIdx.x != first_or_last(mass > 0.0 && s + mass > target, mass > 0.0, itmp)) return;
-  int id = -1;
-  float at = 0.f;
-  bool done = false;
-#pragma unroll
-  for (int i = 0; i < kCols; ++i) {
-    if (!done && e[i] > 0.0) id = c0 + i, at = v[i];
-    s += e[i];
-    done = done || (e[i] > 0.0 && s > target);
-  }
-  g.ids[row] = id;
-  g.logp[row] = (float)(((double)at - (double)max) * r.k * kLn2D) - log_fast(g.open ? (float)total : st.sum);
+  cut_counted(sh, own, g, row, a);
 }
 
 // How a call is cut up. Two blocks a CU, so want = 2 CUs / rows blocks a row; runs as long as they can be (each costs a
@@ -1297,7 +1545,7 @@ Shape shape_of(int64_t rows, int64_t cols, int64_t cus) {
 }
 
 struct Layout {
-  size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, run_ref, hist, cuts, total;
+  size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, run_ref, hist, cuts, list, listed, total;
 };
 Layout layout_of(int64_t rows, const Shape& shape, bool cuts, bool bf16) {
   const int64_t runs = shape.runs, split = shape.split;
@@ -1317,6 +1565,8 @@ Layout layout_of(int64_t rows, const Shape& shape, bool cuts, bool bf16) {
   if (cuts) {
     l.quarters = take((size_t)(rows * runs) * 4 * sizeof(float));
     l.cuts = take((size_t)rows * sizeof(Cut));
+    l.list = take((size_t)(rows * split) * kPartList * sizeof(Listed));
+    l.listed = take((size_t)(rows * split) * sizeof(uint32_t));
     if (split > 1) l.hist = take((size_t)(rows * split) * (bf16 ? sizeof(Hist<__bf16>) : sizeof(Hist<float>)));
   }
   l.total = at;
@@ -1395,47 +1645,48 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   g.run_ref = (float*)(ws + l.run_ref);
   g.hist = ws + l.hist;
   g.cuts = (Cut*)(ws + l.cuts);
-  auto launch = [&](auto tag) {
+  g.list = (Listed*)(ws + l.list);
+  g.listed = (uint32_t*)(ws + l.listed);
+  // Lists: bf16 rows with a top-k each are counted instead, which takes one launch (and reading) fewer than the scan and
+  // the counts or lists that the row's own k asks for.
+  g.lists = !(top_k_rows && dtype == kBF16);
+  const bool all_listed = !top_k_rows && top_k > 0 && top_k < cols && top_k <= list_most(g.runs);
+  const hipStream_t st = (hipStream_t)stream;
+  const dim3 parts((unsigned)(rows * split)), each((unsigned)rows);
+  const auto run = [&](void (*kernel)(SampleArgs), const dim3& grid, const char* name) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kLanes), 0, st, g);
+    return check_launch(name);
+  };
+  auto launch = [&](auto tag) -> int {
     using T = decltype(tag);
-    const hipStream_t st = (hipStream_t)stream;
-    const dim3 parts((unsigned)(rows * split)), each((unsigned)rows);
-    if constexpr (Bins<T>::kExact) {
-      if (cuts) {
-        if (split == 1) {
-          hipLaunchKernelGGL((sample_count_kernel<true>), parts, dim3(kLanes), 0, st, g);
-          if (const int rc = check_launch("sample_count_kernel")) return rc;
-        } else {
-          hipLaunchKernelGGL((sample_count_kernel<false>), parts, dim3(kLanes), 0, st, g);
-          if (const int rc = check_launch("sample_count_kernel")) return rc;
-          hipLaunchKernelGGL(sample_count_cut_kernel, each, dim3(kLanes), 0, st, g);
-          if (const int rc = check_launch("sample_count_cut_kernel")) return rc;
-        }
-      }
-    }
+    constexpr bool kCounts = Bins<T>::kExact;
+    int rc = HK_OK;
     if (!masses) {
-      hipLaunchKernelGGL((sample_open_kernel<T>), parts, dim3(kLanes), 0, st, g);
-      if (const int rc = check_launch("sample_open_kernel")) return rc;
-    } else if (!Bins<T>::kExact || !cuts) {
-      hipLaunchKernelGGL((sample_scan_kernel<T>), parts, dim3(kLanes), 0, st, g);
-      if (const int rc = check_launch("sample_scan_kernel")) return rc;
+      rc = run(sample_open_kernel<T>, parts, "sample_open_kernel");
+    } else if (!kCounts || !cuts || all_listed) {
+      rc = run(sample_scan_kernel<T>, parts, "sample_scan_kernel");
     }
-    if constexpr (!Bins<T>::kExact) {
-      if (cuts) {
-        if (split == 1) hipLaunchKernelGGL((sample_hist_kernel<T, true>), parts, dim3(kLanes), 0, st, g);
-        else hipLaunchKernelGGL((sample_hist_kernel<T, false>), parts, dim3(kLanes), 0, st, g);
-        if (const int rc = check_launch("sample_hist_kernel")) return rc;
-        if (split > 1) {
-          hipLaunchKernelGGL((sample_cut_kernel<T>), each, dim3(kLanes), 0, st, g);
-          if (const int rc = check_launch("sample_cut_kernel")) return rc;
-        }
+    if (rc != HK_OK) return rc;
+    if (all_listed) {
+      rc = run(sample_list_kernel<T>, parts, "sample_list_kernel");
+      return rc != HK_OK ? rc : run(sample_draw_kernel<T>, each, "sample_draw_kernel");
+    }
+    if (cuts) {
+      if constexpr (kCounts) {
+        rc = run(split == 1 ? sample_count_kernel<true> : sample_count_kernel<false>, parts, "sample_count_kernel");
+        if (rc == HK_OK && split > 1) rc = run(sample_count_cut_kernel, each, "sample_count_cut_kernel");
+      } else {
+        auto bins = [&](auto mixed) {
+          constexpr bool kMixed = decltype(mixed)::value;
+          const int bad = run(split == 1 ? sample_hist_kernel<T, true, kMixed> : sample_hist_kernel<T, false, kMixed>,
+                              parts, "sample_hist_kernel");
+          return bad != HK_OK || split == 1 ? bad : run(sample_cut_kernel<T, kMixed>, each, "sample_cut_kernel");
+        };
+        rc = top_k_rows ? bins(std::true_type{}) : bins(std::false_type{});
       }
     }
-    if (masses) {
-      hipLaunchKernelGGL((sample_mass_kernel<T>), parts, dim3(kLanes), 0, st, g);
-      if (const int rc = check_launch("sample_mass_kernel")) return rc;
-    }
-    hipLaunchKernelGGL((sample_pick_kernel<T>), each, dim3(kLanes), 0, st, g);
-    return check_launch("sample_pick_kernel");
+    if (rc == HK_OK && masses) rc = run(sample_mass_kernel<T>, parts, "sample_mass_kernel");
+    return rc != HK_OK ? rc : run(sample_pick_kernel<T>, each, "sample_pick_kernel");
   };
   if (dtype == kF32) return launch(float{});
   if (dtype == kF16) return launch(_Float16{});

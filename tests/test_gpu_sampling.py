@@ -313,3 +313,44 @@ def test_bf16_values_outside_the_bins_of_one_value():
                dict(top_p=0.999), dict(temperature=0.03, top_p=0.9), dict(top_k=2000, top_p=0.6, min_p=1e-3),
                dict(temperature=200.0, top_p=0.7)):
         _check(x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 24, 300])
+def test_few_kept_of_many(dtype, rows):
+    """top-k small enough for a list of candidates, up to where it is not, for one k and a k each."""
+    V = 20011
+    x, u, g = _rows(rows, V, dtype, seed=rows)
+    for k in (1, 2, 50, 160, 161, 207, 208, 209, 257):
+        _check(x, u, top_k=k)
+    _check(x, u, top_k=50, top_p=0.9, min_p=0.01)
+    _check(x, u, top_k=208, top_p=0.7, temperature=2.5)
+    k = torch.randint(1, 230, (rows,), generator=g)
+    _check(x, u, top_k=k, top_p=0.95)
+    _check(x, u, top_k=k * (torch.arange(rows) % 3 > 0), min_p=torch.rand(rows, generator=g) * 0.1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40009, 151936])
+def test_more_candidates_than_a_list_holds(dtype, V):
+    """Ties at the k-th logit: more than a list holds, in one part of a row and over all of them, and just as many."""
+    g = torch.Generator().manual_seed(V)
+    x = (0.5 * torch.randn(10, V, generator=g)).clamp(-4, 2.5).to(dtype)
+    x[0] = 1.0
+    x[1, :5000] = 3.0
+    x[2, torch.randperm(V, generator=g)[:900]] = 3.0
+    x[3, torch.randperm(V, generator=g)[:768]] = 3.0
+    x[4, torch.randperm(V, generator=g)[:769]] = 3.0
+    x[5, -513:] = 3.0
+    x[6, :512] = 3.0
+    x[7] = torch.finfo(dtype).min
+    x[8, 3::7] = -math.inf
+    x[8, 5::7] = math.nan
+    x[9, 40:] = -math.inf
+    u = torch.rand(10, generator=g)
+    for kw in (dict(top_k=60), dict(top_k=60, top_p=0.6), dict(top_k=1), dict(top_k=200, min_p=0.2),
+               dict(top_k=torch.full((10,), 77), top_p=0.9)):
+        _check(x, u, **kw)
+    many = torch.arange(300) % 10
+    _check(x[many, :40009], u[many], top_k=60, top_p=0.8)
+    _check(x[many, :40009], u[many], top_k=torch.full((300,), 33))
