@@ -35,15 +35,20 @@
 //   cut    the bins of a row's blocks together; the bin that holds the cut; if
 //          several values may lie in it, the same over ranges of ordered keys,
 //          11 bits at a time, until one is left: x* and how many ties are kept.
-//          With one block a row this ends the launch before.
+//          With one block a row this ends the launch before. If the bin has 512
+//          logits or less and there is one filter, mass lists them and pick finds
+//          the cut in their order instead: a block takes 25 to 45 us to read a
+//          row of 151936 fp32 logits, mass reads them anyway, and pick takes 10 us
+//          more (256 such rows with top-p: 176 us, 193 before).
 //   mass   the kept mass of each run
 //   pick   the run that u * total falls into, and the token inside it
 //
 // What bounds it: the first pass of 256 rows of 151936 bf16 logits (78 MB) runs
 // at HBM's rate (scan 15 us); the bins' LDS atomics (count 23 us) and the mass
 // table's LDS gathers (mass 34 us, 33 cycles a wave's) are LDS-bound, cut, draw
-// and pick (11, 7 and 7 us) chains of latencies. 77 us in all with top-p, 34 without
-// filters; few rows are bound by those chains, 4 to 14 us a launch.
+// and pick (11, 7 and 7 us) chains of latencies. 77 us in all with top-p, 34
+// without filters; few rows are bound by those chains, 4 to 14 us a launch. fp32
+// and fp16 pay for e^(z - max) in fp64 in hist and mass (50 and 57 us with top-p).
 //
 // Masses are fp64: with 32-bit ones the running sums of a flat row of 1e5
 // tokens (steps of 1e-5 of the total) would be off by a percent of a step, and
@@ -75,9 +80,12 @@ constexpr double kTempMin = 0x1p-64, kTempMax = 0x1p64;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 constexpr int kGroups = 256;          // maxima that a bound on the k-th logit is taken from
 // Rows of few kept logits go by a list of those at or above that bound: for k = 208 of 256 groups it has about
-// 256 ln(256 / 48) = 430 of them, for k = 50 some 56.
+// 256 ln(256 / 48) = 430 of them, for k = 50 some 56. (64 x 151936 bf16: k = 20 25 us, 208 37; by bins k = 209 40.)
 constexpr int kListMost = 208;        // k of such a row at most
 constexpr int kPartList = 512, kList = 768;  // room for a block's, and a row's
+// columns at least: the lists then have half the bytes of the logits at most. 512 rows of 8192 with k = 50 take 27 us,
+// by bins 40 (bf16) and 47 (fp32).
+constexpr int kListCols = 8192;
 __host__ __device__ constexpr int list_most(int runs) { return 4 * runs < kListMost ? 4 * runs : kListMost; }
 
 // A setting of every row, or one each.
@@ -125,11 +133,16 @@ template <typename T> struct Hist {
   uint32_t count[Bins<T>::kCount];
 };
 // A cut: logits above x are kept, and the first `ties` of those equal to x
-// (of `equal` in the row; all of them if ties >= equal).
+// (of `equal` in the row; all of them if ties >= equal). A cut inside `bin`
+// (if that is not -1) is left to the pick: the logits of the bins before it
+// are kept, and of its own, which are x or more, the first `target` in order,
+// or as many as have that mass.
 struct Cut {
   float x;
   uint32_t ties, equal;
   uint32_t count;  // logits kept
+  u64 target = 0;
+  int bin = -1;
 };
 struct Listed {
   float x;
@@ -401,7 +414,7 @@ struct Start {
   }
   __device__ __forceinline__ void cut_min_p() {
     const float f = least_of_min_p(a, max);
-    if (f > cut.x) cut = {f, 0xffffffffu, 0, cut.count};
+    if (f > cut.x) cut.x = f, cut.ties = 0xffffffffu, cut.equal = 0;
   }
 };
 
@@ -796,8 +809,9 @@ struct Row {
   }
 
   // The cut after `count` logits (by count) or at mass `tau` (fixed point), and the mass that it keeps.
+  // If the bin's logits fit into a list and `defer`, the cut stays inside the bin.
   __device__ __forceinline__ Cut find_cut(CutShared<T>& sh, const Share<B::kCount>& share, bool by_count, uint32_t count,
-                                          u64 tau, bool masses, u64* kept) const {
+                                          u64 tau, bool masses, bool defer, u64* kept) const {
     share.find(sh, by_count, count, tau);
     const int bin = sh.bin;
     uint32_t cnt = sh.cnt_before;
@@ -807,6 +821,10 @@ struct Row {
     uint32_t equal = 0;
     if (one_value(bin, &klo, &khi, &value)) {
       equal = sh.hist.count[bin];
+    } else if (!B::kExact && defer && sh.hist.count[bin] <= (uint32_t)kPartList) {
+      const float least = value_of<T>(klo);
+      *kept = 0;
+      return {least == least ? least : -INFINITY, 0xffffffffu, 0, cnt, by_count ? count - cnt : tau - above, bin};
     } else {
       // 32 bits of key in turns of 11
 #pragma unroll 1
@@ -875,12 +893,13 @@ struct Row {
   }
 
   // The row's cut by top-k and top-p, from sh.hist.
-  __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a) const {
+  __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a, bool defer) const {
     const Share<B::kCount> share(
         sh.hist.count, [&](int b, uint32_t c) { return a.by_p ? mass_of_bin(sh.hist, b, c) : 0; }, sh);
-    return find(sh, a, share);
+    return find(sh, a, share, defer);
   }
-  __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a, const Share<B::kCount>& share) const {
+  // (a top-p after a top-k needs the mass that this keeps)
+  __device__ __forceinline__ Cut find(CutShared<T>& sh, const Asked& a, const Share<B::kCount>& share, bool defer) const {
     u64 total = share.all_mass;
     Cut cut = {INFINITY, 0, 0, 0};
     // by count, then by mass of what that kept
@@ -888,7 +907,7 @@ struct Row {
     for (int turn = a.by_k ? 0 : 1; turn < (a.by_p ? 2 : 1); ++turn) {
       const u64 tau = ::min(total, ::max((u64)1, (u64)ceil(fmax(a.top_p, 0.0) * (double)total)));
       u64 kept;
-      const Cut c = find_cut(sh, share, turn == 0, (uint32_t)a.top_k, tau, a.by_p, &kept);
+      const Cut c = find_cut(sh, share, turn == 0, (uint32_t)a.top_k, tau, a.by_p, defer && a.by_k != a.by_p, &kept);
       if (turn == 0 || !a.by_k || c.x > cut.x) cut = c;
       else if (c.x == cut.x && c.ties < cut.ties) cut.ties = c.ties, cut.count = c.count;
       total = kept;
@@ -897,9 +916,80 @@ struct Row {
   }
 };
 
+// ---- lists --------------------------------------------------------------------
+// A block's list: logits and their columns, in any order.
+struct ListShared {
+  uint32_t n;
+  Listed list[kPartList];
+  __device__ __forceinline__ void clear() {
+    if (threadIdx.x == 0) n = 0;
+    __syncthreads();
+  }
+  __device__ __forceinline__ void add(float x, int col) {
+    const uint32_t at = atomicAdd(&n, 1u);
+    if (at < (uint32_t)kPartList) list[at] = {x, col};
+  }
+  __device__ __forceinline__ void write(const SampleArgs& g, int64_t block) const {
+    __syncthreads();
+    for (int i = threadIdx.x; i < (int)min(n, (uint32_t)kPartList); i += kLanes) g.list[block * kPartList + i] = list[i];
+    if (threadIdx.x == 0) g.listed[block] = n;
+  }
+};
+// A row's lists in order, x descending and then by column; returns how many, -1 if a block's list or the row's has not
+// room for all. Ends with a barrier.
+struct OrderShared {
+  u64 key[kList];  // larger x, then lower column, first
+  uint32_t rank[kList];
+  float x[kList];  // in order
+  int col[kList];
+};
+__device__ __forceinline__ int order_listed(const SampleArgs& g, int64_t row, OrderShared& sh) {
+  const int lane = threadIdx.x % kWave, t = threadIdx.x;
+  const uint32_t in_part = lane < g.split ? g.listed[row * g.split + lane] : 0;
+  const uint32_t incl = wave_scan(in_part);
+  const int n = (int)of_lane63(incl);
+  if (__any(in_part > (uint32_t)kPartList) || n > kList) return -1;
+  int part = 0;
+  uint32_t before_part = 0;
+#pragma unroll 1
+  for (int i = 0; i < g.split - 1; ++i) {
+    const uint32_t upto = of_lane(incl, i);
+    if ((uint32_t)t >= upto) part = i + 1, before_part = upto;
+  }
+  Listed mine = {0.f, 0};
+  if (t < n) {
+    mine = g.list[(row * g.split + part) * kPartList + (t - before_part)];
+    sh.key[t] = (u64)key_of<float>(mine.x) << 32 | (uint32_t)~mine.col;
+    sh.rank[t] = 0;
+  }
+  __syncthreads();
+  // the rank of each, by comparison with all; the threads share them out
+  int width = kWave;
+  while (width < n) width *= 2;
+  const int i = t & (width - 1), q = t / width, each = (n + kLanes / width - 1) / (kLanes / width);
+  if (i < n) {
+    const u64 key = sh.key[i];
+    uint32_t rank = 0;
+#pragma unroll 4
+    for (int j = q * each; j < min(n, (q + 1) * each); ++j) rank += sh.key[j] > key ? 1 : 0;
+    if (rank) atomicAdd(&sh.rank[i], rank);
+  }
+  __syncthreads();
+  if (t < n) {
+    const uint32_t r = sh.rank[t];
+    sh.x[r] = mine.x;
+    sh.col[r] = mine.col;
+  }
+  __syncthreads();
+  return n;
+}
+
 // ---- mass -------------------------------------------------------------------
 template <typename T> struct MassShared {
-  double table[Bins<T>::kExact ? Bins<__bf16>::kUsed : 1];
+  ListShared list;  // of the bin that a cut is inside of
+};
+template <> struct MassShared<__bf16> {
+  double table[Bins<__bf16>::kUsed];
 };
 // The kept masses of one block's runs (part of split).
 template <typename T>
@@ -943,6 +1033,30 @@ __device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int
       return;
     }
   }
+  if constexpr (!kTable) {
+    if (cut.bin >= 0) {
+      sh.list.clear();
+      each_run(
+          r.x, g.cols, g.run_cols, g.runs, first, waves,
+          [&](const Pack<T, VEC>& p, int c) {
+            float v[VEC];
+            unpack(p, v);
+            float most = v[0];
+#pragma unroll
+            for (int i = 1; i < VEC; ++i) most = fmaxf(most, v[i]);
+            if (!__any(most >= cut.x)) return;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+              const int bin = v[i] >= cut.x ? r.bin_of(v[i]) : cut.bin + 1;
+              mass += bin < cut.bin ? r.mass(v[i]) : 0.0;
+              if (bin == cut.bin && c + i < g.cols) sh.list.add(v[i], c + i);
+            }
+          },
+          done);
+      sh.list.write(g, row * split + part);
+      return;
+    }
+  }
   each_run(
       r.x, g.cols, g.run_cols, g.runs, first, waves,
       [&](const Pack<T, VEC>& p, int) {
@@ -975,9 +1089,50 @@ struct PickShared {
   float ftmp[kWaves];
   int itmp[2 * kWaves], run;
 };
+// A cut inside a bin: orders the bin's list, adds the masses that are kept to their runs', and leaves the last kept logit
+// and its column as the cut. The masses of a run are added in that order by one thread, so calls repeat.
+struct InsideShared : OrderShared {
+  double e[kPartList];
+  int run[kPartList];
+  u64 ltmp[kWaves];
+  int last;
+};
+template <typename T>
+__device__ __forceinline__ void cut_inside(const SampleArgs& g, int64_t row, Start& st, int* last_col, InsideShared& sh) {
+  const Row<T> r(g, row, st.a, st.max);
+  const int n = order_listed(g, row, sh), t = threadIdx.x;
+  const float x = t < n ? sh.x[t] : -INFINITY;
+  const int run = t < n ? sh.col[t] / g.run_cols : -1;
+  const double e = t < n ? r.mass(x) : 0.0;
+  u64 all;
+  const u64 before = st.a.by_k ? (u64)t : block_before<u64>(t < n ? r.fixed(e) : 0, sh.ltmp, &all);
+  const bool keep = t < n && before < st.cut.target;
+  if (t == 0) sh.last = -1;
+  __syncthreads();
+  if (t < n) sh.e[t] = e, sh.run[t] = keep ? run : -1;
+  const u64 kept_here = __ballot(keep);
+  if (keep && t % kWave == 63 - __builtin_clzll(kept_here)) atomicMax(&sh.last, t);
+  __syncthreads();
+  const int last = sh.last;
+  if (keep) {
+    double sum = 0.0;
+    bool first = true;
+#pragma unroll 4
+    for (int j = 0; j <= last; ++j) {
+      const bool same = sh.run[j] == run;
+      sum += same ? sh.e[j] : 0.0;
+      first = first && !(same && j < t);
+    }
+    if (first) g.run_mass[row * g.runs + run] += sum;
+  }
+  // (none is listed if min-p cuts above the bin: x is its least then)
+  if (last >= 0) st.cut.x = sh.x[last], *last_col = sh.col[last];
+  __syncthreads();
+}
 // The row's token from the masses of its runs; `start` gives its Start.
 template <typename T, typename S>
-__device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& start, PickShared& sh) {
+__device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& start, PickShared& sh,
+                                         InsideShared* inside) {
   constexpr int kCols = 2;  // columns a thread, in order: runs of up to 2048
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
   const double* run_mass = g.run_mass + row * g.runs;
@@ -987,7 +1142,7 @@ __device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& s
   const int r0 = min(g.runs, (int)threadIdx.x * per), r1 = min(g.runs, r0 + per);
   // the first run's records, on the way while the row's start is put together (mostly there is no other)
   const int any_run = min(r0, g.runs - 1);
-  const double mass0 = run_mass[any_run];
+  double mass0 = run_mass[any_run];
   const uint32_t ties0 = run_ties[any_run];
   const float max0 = run_max[any_run], ref0 = run_ref[any_run];
   Start st = start();
@@ -1009,6 +1164,13 @@ __device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& s
   if (!fine) {
     if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
     return;
+  }
+  int last_col = g.cols;  // of the logits equal to the cut
+  if constexpr (!Bins<T>::kExact) {
+    if (inside && !g.open && st.cut.bin >= 0) {
+      cut_inside<T>(g, row, st, &last_col, *inside);
+      mass0 = run_mass[any_run];
+    }
   }
   const float max = st.max;
   const Row<T> r(g, row, st.a, st.max);
@@ -1075,7 +1237,7 @@ __device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& s
   mass = 0.0;
 #pragma unroll
   for (int i = 0; i < kCols; ++i) {
-    bool keep = v[i] >= cut.x;
+    bool keep = v[i] > cut.x || (v[i] == cut.x && c0 + i <= last_col);
     if (!all_ties && v[i] == cut.x) keep = rank++ < cut.ties;
     e[i] = keep ? r.mass(v[i]) : 0.0;
     mass += e[i];
@@ -1101,7 +1263,8 @@ __global__ __launch_bounds__(kLanes) void sample_pick_kernel(SampleArgs g) {
   __shared__ PickShared sh;
   const int64_t row = blockIdx.x;
   if (g.lists && asked(g, row).by_list) return;
-  pick_row<T>(g, row, [&] { return Start(g, row, true); }, sh);
+  __shared__ InsideShared inside;  // (bf16 has no use for it, and no room is taken)
+  pick_row<T>(g, row, [&] { return Start(g, row, true); }, sh, &inside);
 }
 
 // ---- list -------------------------------------------------------------------
@@ -1137,17 +1300,12 @@ __device__ __forceinline__ float least_of_top_k(const SampleArgs& g, int64_t row
 }
 
 // Lists the logits of one block's runs that reach `least` (all finite ones if that is -inf), in any order.
-struct ListShared {
-  uint32_t n;
-  Listed list[kPartList];
-};
 template <typename T>
 __device__ __forceinline__ void list_block(const T* x, const SampleArgs& g, int64_t row, int part, float least,
                                            ListShared& sh) {
   constexpr int VEC = 16 / sizeof(T);
   const float bound = fmaxf(least, -3.402823466e38f);
-  if (threadIdx.x == 0) sh.n = 0;
-  __syncthreads();
+  sh.clear();
   each_run(
       x, g.cols, g.run_cols, g.runs, part * kWaves + (int)threadIdx.x / kWave, g.split * kWaves,
       [&](const Pack<T, VEC>& p, int c) {
@@ -1159,25 +1317,15 @@ __device__ __forceinline__ void list_block(const T* x, const SampleArgs& g, int6
         if (!__any(most >= bound)) return;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          if (v[i] >= bound) {
-            const uint32_t at = atomicAdd(&sh.n, 1u);
-            if (at < (uint32_t)kPartList) sh.list[at] = {v[i], c + i};
-          }
+          if (v[i] >= bound) sh.add(v[i], c + i);
         }
       },
       [](int) {});
-  __syncthreads();
-  const int64_t block = row * g.split + part;
-  for (int i = threadIdx.x; i < (int)min(sh.n, (uint32_t)kPartList); i += kLanes) g.list[block * kPartList + i] = sh.list[i];
-  if (threadIdx.x == 0) g.listed[block] = sh.n;
+  sh.write(g, row * g.split + part);
 }
 
 // Draws a row's token from its list; false if that has not room for all.
-struct DrawShared {
-  u64 key[kList];       // of the listed: larger x, then lower column, first
-  uint32_t rank[kList];
-  float x[kList];       // in that order
-  int col[kList];
+struct DrawShared : OrderShared {
   double e[kListMost];  // of the kept, by column
   int from[kListMost];
   double dtmp[kWaves];
@@ -1185,48 +1333,13 @@ struct DrawShared {
 };
 __device__ __forceinline__ bool draw_listed(const SampleArgs& g, int64_t row, const Start& st, DrawShared& sh) {
   const Asked& a = st.a;
-  const int lane = threadIdx.x % kWave, t = threadIdx.x;
+  const int t = threadIdx.x;
   const float u = g.u[row];
-  const uint32_t in_part = lane < g.split ? g.listed[row * g.split + lane] : 0;
-  const uint32_t incl = wave_scan(in_part), n = of_lane63(incl);
-  if (__any(in_part > (uint32_t)kPartList) || n > (uint32_t)kList) return false;
-  int part = 0;
-  uint32_t before_part = 0;
-#pragma unroll 1
-  for (int i = 0; i < g.split - 1; ++i) {
-    const uint32_t upto = of_lane(incl, i);
-    if ((uint32_t)t >= upto) part = i + 1, before_part = upto;
-  }
-  Listed mine = {0.f, 0};
-  if (t < (int)n) {
-    mine = g.list[(row * g.split + part) * kPartList + (t - before_part)];
-    sh.key[t] = (u64)key_of<float>(mine.x) << 32 | (uint32_t)~mine.col;
-    sh.rank[t] = 0;
-  }
+  const int n = order_listed(g, row, sh);
+  if (n < 0) return false;
   if (t < kListMost) sh.e[t] = 0.0;
-  __syncthreads();
-  // the rank of each, by comparison with all; the threads share them out
-  {
-    int width = kWave;
-    while (width < (int)n) width *= 2;
-    const int i = t & (width - 1), q = t / width, each = ((int)n + kLanes / width - 1) / (kLanes / width);
-    if (i < (int)n) {
-      const u64 key = sh.key[i];
-      uint32_t rank = 0;
-#pragma unroll 4
-      for (int j = q * each; j < min((int)n, (q + 1) * each); ++j) rank += sh.key[j] > key ? 1 : 0;
-      if (rank) atomicAdd(&sh.rank[i], rank);
-    }
-  }
-  __syncthreads();
-  if (t < (int)n) {
-    const uint32_t r = sh.rank[t];
-    sh.x[r] = mine.x;
-    sh.col[r] = mine.col;
-  }
-  __syncthreads();
   // the filters keep a prefix of that order
-  const int k = min((int)a.top_k, (int)n);
+  const int k = min((int)a.top_k, n);
   const float x = t < k ? sh.x[t] : -INFINITY;
   const int col = t < k ? sh.col[t] : 0x7fffffff;
   const double e = exp2_product((double)x - (double)st.max, a.k);
@@ -1256,8 +1369,8 @@ __device__ __forceinline__ bool draw_listed(const SampleArgs& g, int64_t row, co
 }
 
 // What a row that goes by a list may need: the list is short of room if many logits equal the bound, and then one block
-// goes the way of the others (cut, mass, pick) for the row (160 us for 64 rows of 151936 equal bf16 logits; rows with 512
-// logits equal to the k-th are none that a model gives).
+// goes the way of the others (cut, mass, pick) for the row (160 us for 64 rows of 151936 equal bf16 logits, 26 for
+// random ones).
 template <typename T>
 union __align__(16) ListedShared {
   ListShared list;
@@ -1274,12 +1387,12 @@ __device__ __forceinline__ void end_listed(const SampleArgs& g, int64_t row, Sta
   if (draw_listed(g, row, st, sh.draw)) return;
   const Row<T> r(g, row, st.a, st.max);
   r.fill(sh.cut.hist, 0, 1, st.a.by_p);
-  st.cut = r.find(sh.cut, st.a);
+  st.cut = r.find(sh.cut, st.a, false);
   st.cut_min_p();
   __syncthreads();
   mass_block<T>(g, row, 0, 1, st, sh.rest.mass);
   __syncthreads();
-  pick_row<T>(g, row, [&] { return st; }, sh.rest.pick);
+  pick_row<T>(g, row, [&] { return st; }, sh.rest.pick, nullptr);
 }
 
 // A call whose rows all go by lists.
@@ -1345,7 +1458,7 @@ __global__ __launch_bounds__(kLanes) void sample_hist_kernel(SampleArgs g) {
   }
   r.fill(sh.cut.hist, part, g.split, st.a.by_p);
   if constexpr (WHOLE) {
-    const Cut cut = r.find(sh.cut, st.a);
+    const Cut cut = r.find(sh.cut, st.a, g.cols >= kListCols);
     if (threadIdx.x == 0) g.cuts[row] = cut;
   } else {
     __syncthreads();
@@ -1397,7 +1510,7 @@ __global__ __launch_bounds__(kLanes) void sample_cut_kernel(SampleArgs g) {
     for (int i = 2 * threadIdx.x; i < Bins<T>::kMasses; i += 2 * kLanes)
       *reinterpret_cast<u64x2*>(&sh.hist.mass[i]) =
           sum_parts<u64x2>((const char*)&from->mass[i], sizeof(Hist<T>), g.split);
-  const Cut cut = r.find(sh, st.a);
+  const Cut cut = r.find(sh, st.a, g.cols >= kListCols);
   if (threadIdx.x == 0) g.cuts[row] = cut;
 }
 
@@ -1482,7 +1595,7 @@ __device__ __forceinline__ void cut_counted(CutShared<__bf16>& sh, CountShared& 
     const Share<B::kCount> share(
         sh.hist.count, [&](int b, uint32_t c) { return r.mass_of_bin(sh.hist, b, c); }, sh);
     if (!again) sum = (float)((double)share.all_mass / (double)r.fixed(1.0));
-    if (cuts) cut = r.find(sh, a, share);
+    if (cuts) cut = r.find(sh, a, share, false);
   }
   if (threadIdx.x < g.split) {
     g.part_max[row * g.split + threadIdx.x] = threadIdx.x == 0 ? max : -INFINITY;
@@ -1547,7 +1660,7 @@ Shape shape_of(int64_t rows, int64_t cols, int64_t cus) {
 struct Layout {
   size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, run_ref, hist, cuts, list, listed, total;
 };
-Layout layout_of(int64_t rows, const Shape& shape, bool cuts, bool bf16) {
+Layout layout_of(int64_t rows, int64_t cols, const Shape& shape, bool cuts, bool bf16) {
   const int64_t runs = shape.runs, split = shape.split;
   Layout l = {};
   size_t at = 0;
@@ -1563,10 +1676,12 @@ Layout layout_of(int64_t rows, const Shape& shape, bool cuts, bool bf16) {
   l.part_max = take((size_t)(rows * split) * sizeof(float));
   l.part_sum = take((size_t)(rows * split) * sizeof(float));
   if (cuts) {
-    l.quarters = take((size_t)(rows * runs) * 4 * sizeof(float));
     l.cuts = take((size_t)rows * sizeof(Cut));
-    l.list = take((size_t)(rows * split) * kPartList * sizeof(Listed));
-    l.listed = take((size_t)(rows * split) * sizeof(uint32_t));
+    if (cols >= kListCols) {
+      l.quarters = take((size_t)(rows * runs) * 4 * sizeof(float));
+      l.list = take((size_t)(rows * split) * kPartList * sizeof(Listed));
+      l.listed = take((size_t)(rows * split) * sizeof(uint32_t));
+    }
     if (split > 1) l.hist = take((size_t)(rows * split) * (bf16 ? sizeof(Hist<__bf16>) : sizeof(Hist<float>)));
   }
   l.total = at;
@@ -1583,7 +1698,7 @@ extern "C" {
 size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int dtype, int device) {
   if (rows < 0 || rows >= (1LL << 31) || cols <= 0 || cols > (1 << 30)) return 0;
   const int cus = cu_count(device);
-  return std::max<size_t>(256, layout_of(rows, shape_of(rows, cols, cus > 0 ? cus : 256), cuts != 0, dtype == kBF16).total);
+  return std::max<size_t>(256, layout_of(rows, cols, shape_of(rows, cols, cus > 0 ? cus : 256), cuts != 0, dtype == kBF16).total);
 }
 
 int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int64_t rows, int64_t cols, int64_t ld,
@@ -1612,7 +1727,7 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   HK_REQUIRE(rows * split < (1LL << 32) / kLanes, "rows=%lld too many for one launch", (long long)rows);
   const bool cuts = top_k_rows || (top_k > 0 && top_k < cols) || top_p_rows || top_p < 1;
   const bool masses = cuts || min_p_rows || min_p > 0;
-  const Layout l = layout_of(rows, shape, cuts, dtype == kBF16);
+  const Layout l = layout_of(rows, cols, shape, cuts, dtype == kBF16);
   HK_REQUIRE(workspace_bytes >= l.total, "workspace too small: need %zu bytes, got %zu", l.total, workspace_bytes);
   char* ws = (char*)workspace;
   SampleArgs g = {};
@@ -1649,8 +1764,8 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   g.listed = (uint32_t*)(ws + l.listed);
   // Lists: bf16 rows with a top-k each are counted instead, which takes one launch (and reading) fewer than the scan and
   // the counts or lists that the row's own k asks for.
-  g.lists = !(top_k_rows && dtype == kBF16);
-  const bool all_listed = !top_k_rows && top_k > 0 && top_k < cols && top_k <= list_most(g.runs);
+  g.lists = cols >= kListCols && !(top_k_rows && dtype == kBF16);
+  const bool all_listed = g.lists && !top_k_rows && top_k > 0 && top_k < cols && top_k <= list_most(g.runs);
   const hipStream_t st = (hipStream_t)stream;
   const dim3 parts((unsigned)(rows * split)), each((unsigned)rows);
   const auto run = [&](void (*kernel)(SampleArgs), const dim3& grid, const char* name) {

@@ -354,3 +354,34 @@ def test_more_candidates_than_a_list_holds(dtype, V):
     many = torch.arange(300) % 10
     _check(x[many, :40009], u[many], top_k=60, top_p=0.8)
     _check(x[many, :40009], u[many], top_k=torch.full((300,), 33))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 24, 300])
+def test_one_filter_over_many_kept(dtype, rows):
+    """One filter whose cut lies among many different logits, next to min-p and ties at the cut."""
+    V = 30011
+    x, u, g = _rows(rows, V, dtype, seed=rows + 1, lo=0.3, hi=4.0)
+    some = torch.rand(rows, V, generator=g) < 0.02
+    x = torch.where(some, x[:, :1].expand(rows, V), x)  # 600 equal logits somewhere in the row
+    for kw in (dict(top_p=0.95), dict(top_p=0.5), dict(top_k=3000), dict(top_k=301), dict(top_k=3000, min_p=0.001),
+               dict(top_p=0.9, min_p=0.05), dict(top_p=0.7, temperature=3.0), dict(top_k=25000),
+               dict(top_p=torch.rand(rows, generator=g)), dict(top_k=torch.randint(1, V, (rows,), generator=g))):
+        _check(x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cuts_among_masked_tokens(dtype):
+    """A top-k larger than what is left, masks of the lowest value, ties of all a mask leaves."""
+    V = 9001
+    x, u, g = _rows(8, V, dtype, seed=9)
+    x[0, 300:] = -math.inf
+    x[1, 300:] = torch.finfo(dtype).min
+    x[2, :8700] = -math.inf
+    x[3, 400:] = -60.0
+    x[4, 1:] = -math.inf
+    x[5] = -math.inf
+    x[5, ::30] = 2.0
+    x[6] = x[6].abs() * 200
+    for kw in (dict(top_k=400), dict(top_k=8999), dict(top_p=0.999), dict(top_k=500, top_p=0.99), dict(top_k=1000, min_p=0.5)):
+        _check(x, u, **kw)
