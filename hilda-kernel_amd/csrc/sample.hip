@@ -40,13 +40,15 @@
 //          the cut in their order instead: a block takes 25 to 45 us to read a
 //          row of 151936 fp32 logits, mass reads them anyway, and pick takes 10 us
 //          more (256 such rows with top-p: 176 us, 193 before).
-//   mass   the kept mass of each run
+//          Of bf16 rows in few long parts it also tells the part that the
+//          token lies in, by the parts' counts.
+//   mass   the kept mass of each run (of that part)
 //   pick   the run that u * total falls into, and the token inside it
 //
 // What bounds it: the first pass of 256 rows of 151936 bf16 logits (78 MB) runs
 // at HBM's rate (scan 15 us); the bins' LDS atomics (count 23 us) and the mass
-// table's LDS gathers (mass 34 us, 33 cycles a wave's) are LDS-bound, cut, draw
-// and pick (11, 7 and 7 us) chains of latencies. 77 us in all with top-p, 34
+// table's LDS gathers (mass 21 us, 33 cycles a wave's) are LDS-bound, cut, draw
+// and pick (16, 7 and 8 us) chains of latencies. 69 us in all with top-p, 35
 // without filters; few rows are bound by those chains, 4 to 14 us a launch. fp32
 // and fp16 pay for e^(z - max) in fp64 in hist and mass (50 and 57 us with top-p).
 //
@@ -79,6 +81,10 @@ constexpr double kRange = 24;
 constexpr double kTempMin = 0x1p-64, kTempMax = 0x1p64;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 constexpr int kGroups = 256;          // maxima that a bound on the k-th logit is taken from
+// Columns of a part at least for a choice of the part (choose_part takes 6 us; bf16, top-p 0.95 and 0.5, with and without:
+// 256 rows in parts of 76000 71 and 81, 61 and 61 us; 128 of 38000 52 and 56, 48 and 47; 256 of 33000 51 and 53, 48 and 45;
+// 1 of 8000 39 and 33, 37 and 31).
+constexpr int64_t kChooseCols = 36 << 10;
 // Rows of few kept logits go by a list of those at or above that bound: for k = 208 of 256 groups it has about
 // 256 ln(256 / 48) = 430 of them, for k = 50 some 56. (64 x 151936 bf16: k = 20 25 us, 208 37; by bins k = 209 40.)
 constexpr int kListMost = 208;        // k of such a row at most
@@ -133,20 +139,28 @@ template <typename T> struct Hist {
   uint32_t count[Bins<T>::kCount];
 };
 // A cut: logits above x are kept, and the first `ties` of those equal to x
-// (of `equal` in the row; all of them if ties >= equal). A cut inside `bin`
-// (if that is not -1) is left to the pick: the logits of the bins before it
+// (of `equal` in the row; all of them if ties >= equal). A cut inside the bin
+// inside - 1 (0: none) is left to the pick: the logits of the bins before it
 // are kept, and of its own, which are x or more, the first `target` in order,
 // or as many as have that mass.
 struct Cut {
   float x;
   uint32_t ties, equal;
   uint32_t count;  // logits kept
-  u64 target = 0;
-  int bin = -1;
+  u64 target;
+  int inside;
 };
 struct Listed {
   float x;
   int col;
+};
+// The part of a row (of `split`, whose runs lie side by side) that u * total
+// falls into, the kept mass and ties before it and the kept mass of the row;
+// -1: not known.
+struct Chosen {
+  double before, total;
+  uint32_t ties;
+  int part;
 };
 struct SampleArgs {
   int64_t* ids;
@@ -172,6 +186,7 @@ struct SampleArgs {
   float *run_max, *run_ref;    // of an open call: the run's maximum, and the logit whose mass its masses take as 1
   void* hist;                  // Hist<T> [rows][split], split > 1
   Cut* cuts;                   // [rows]
+  Chosen* chosen;              // [rows], or null: no row has one
   Listed* list;                // [rows][split][kPartList]
   uint32_t* listed;            // [rows][split] how many (more than kPartList: not all are there)
 };
@@ -391,6 +406,18 @@ __device__ __forceinline__ float least_of_min_p(const Asked& a, float max) {
   return (double)f < least ? nextafterf(f, INFINITY) : f;
 }
 
+__device__ __forceinline__ void apply_min_p(Cut& cut, const Asked& a, float max) {
+  const float f = least_of_min_p(a, max);
+  if (f > cut.x) cut.x = f, cut.ties = 0xffffffffu, cut.equal = 0;
+}
+// The runs [begin, end) of a part of a row.
+struct Runs {
+  int begin, end;
+};
+__device__ __forceinline__ Runs runs_of(const SampleArgs& g, int part) {
+  return {(int)((int64_t)g.runs * part / g.split), (int)((int64_t)g.runs * (part + 1) / g.split)};
+}
+
 // What the launches after the scan begin with, its loads in flight together: the row's settings, its maximum and sum of
 // e^(z - max) from its blocks' parts (every wave puts them together for itself), and its cut. ok: it has a distribution.
 struct Start {
@@ -413,8 +440,7 @@ struct Start {
     if (with_cut && ok) cut_min_p();
   }
   __device__ __forceinline__ void cut_min_p() {
-    const float f = least_of_min_p(a, max);
-    if (f > cut.x) cut.x = f, cut.ties = 0xffffffffu, cut.equal = 0;
+    apply_min_p(cut, a, max);
   }
 };
 
@@ -824,7 +850,7 @@ struct Row {
     } else if (!B::kExact && defer && sh.hist.count[bin] <= (uint32_t)kPartList) {
       const float least = value_of<T>(klo);
       *kept = 0;
-      return {least == least ? least : -INFINITY, 0xffffffffu, 0, cnt, by_count ? count - cnt : tau - above, bin};
+      return {least == least ? least : -INFINITY, 0xffffffffu, 0, cnt, by_count ? count - cnt : tau - above, bin + 1};
     } else {
       // 32 bits of key in turns of 11
 #pragma unroll 1
@@ -881,7 +907,7 @@ struct Row {
         klo = ::max(klo, khi - ((1u << s) - 1));
       }
     }
-    Cut cut;
+    Cut cut = {};
     cut.x = value;
     cut.equal = equal;
     const u64 each = masses ? fixed(mass(value)) : 0;
@@ -991,10 +1017,10 @@ template <typename T> struct MassShared {
 template <> struct MassShared<__bf16> {
   double table[Bins<__bf16>::kUsed];
 };
-// The kept masses of one block's runs (part of split).
+// The kept masses of one block's share (part of split) of `runs`.
 template <typename T>
-__device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int part, int split, const Start& st,
-                                           MassShared<T>& sh) {
+__device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, const Runs& runs, int part, int split,
+                                           const Start& st, MassShared<T>& sh) {
   constexpr int VEC = 16 / sizeof(T);
   constexpr bool kTable = Bins<T>::kExact;
   const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
@@ -1004,7 +1030,7 @@ __device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int
   auto kept = [&](float v) { return all_ties ? v >= cut.x : v > cut.x; };
   double mass = 0.0;
   uint32_t ties = 0;  // (the wave's)
-  const int first = part * kWaves + wave, waves = split * kWaves;
+  const int first = runs.begin + part * kWaves + wave, waves = split * kWaves;
   auto count_ties = [&](const Pack<T, VEC>& p) {
     if (all_ties) return;
     float v[VEC];
@@ -1019,12 +1045,14 @@ __device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int
     ties = 0;
   };
   if constexpr (kTable) {
-    // few are kept: the table costs more than their polynomials (2 us; 1 in 64 of 38000 logits a block 0.6)
-    if (cut.count > (uint32_t)g.cols / 64) {
+    // The table is as many polynomials as it has bins: worth it for twice as many logits, of which more than a few are
+    // kept.
+    if (cut.count > (uint32_t)g.cols / 64 &&
+        (int64_t)(runs.end - runs.begin) * g.run_cols > (int64_t)split * 2 * Bins<T>::kUsed) {
       const int reach = Bins<T>::of(cut.x);
       fill_table(sh.table, reach, [&](float v) { return v <= st.max && kept(v) ? r.mass(v) : 0.0; });
       each_run(
-          r.x, g.cols, g.run_cols, g.runs, first, waves,
+          r.x, g.cols, g.run_cols, runs.end, first, waves,
           [&](const Pack<T, VEC>& p, int) {
             mass += sum_table(sh.table, p, reach, [&](float y) { return kept(y) ? r.mass(y) : 0.0; });
             count_ties(p);
@@ -1034,10 +1062,11 @@ __device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int
     }
   }
   if constexpr (!kTable) {
-    if (cut.bin >= 0) {
+    if (cut.inside) {
+      const int inside = cut.inside - 1;
       sh.list.clear();
       each_run(
-          r.x, g.cols, g.run_cols, g.runs, first, waves,
+          r.x, g.cols, g.run_cols, runs.end, first, waves,
           [&](const Pack<T, VEC>& p, int c) {
             float v[VEC];
             unpack(p, v);
@@ -1047,9 +1076,9 @@ __device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int
             if (!__any(most >= cut.x)) return;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-              const int bin = v[i] >= cut.x ? r.bin_of(v[i]) : cut.bin + 1;
-              mass += bin < cut.bin ? r.mass(v[i]) : 0.0;
-              if (bin == cut.bin && c + i < g.cols) sh.list.add(v[i], c + i);
+              const int bin = v[i] >= cut.x ? r.bin_of(v[i]) : inside + 1;
+              mass += bin < inside ? r.mass(v[i]) : 0.0;
+              if (bin == inside && c + i < g.cols) sh.list.add(v[i], c + i);
             }
           },
           done);
@@ -1058,7 +1087,7 @@ __device__ __forceinline__ void mass_block(const SampleArgs& g, int64_t row, int
     }
   }
   each_run(
-      r.x, g.cols, g.run_cols, g.runs, first, waves,
+      r.x, g.cols, g.run_cols, runs.end, first, waves,
       [&](const Pack<T, VEC>& p, int) {
         float v[VEC];
         unpack(p, v);
@@ -1079,7 +1108,12 @@ __global__ __launch_bounds__(kLanes) void sample_mass_kernel(SampleArgs g) {
   __shared__ MassShared<T> sh;
   const int64_t row = blockIdx.x / g.split;
   const Start st(g, row, true);
-  if (st.ok && !st.a.by_list) mass_block<T>(g, row, (int)(blockIdx.x % g.split), g.split, st, sh);
+  Runs runs = {0, g.runs};
+  if (Bins<T>::kExact && g.chosen) {
+    const int part = g.chosen[row].part;
+    if (part >= 0) runs = runs_of(g, part);
+  }
+  if (st.ok && !st.a.by_list) mass_block<T>(g, row, runs, (int)(blockIdx.x % g.split), g.split, st, sh);
 }
 
 // ---- pick -------------------------------------------------------------------
@@ -1138,8 +1172,11 @@ __device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& s
   const double* run_mass = g.run_mass + row * g.runs;
   const uint32_t* run_ties = g.run_ties + row * g.runs;
   const float *run_max = g.run_max + row * g.runs, *run_ref = g.run_ref + row * g.runs;
-  const int per = (g.runs + kLanes - 1) / kLanes;  // runs a thread, in order
-  const int r0 = min(g.runs, (int)threadIdx.x * per), r1 = min(g.runs, r0 + per);
+  Chosen from = {0.0, 0.0, 0, -1};
+  if (Bins<T>::kExact && g.chosen) from = g.chosen[row];
+  const Runs runs = from.part >= 0 ? runs_of(g, from.part) : Runs{0, g.runs};
+  const int per = (runs.end - runs.begin + kLanes - 1) / kLanes;  // runs a thread, in order
+  const int r0 = min(runs.end, runs.begin + (int)threadIdx.x * per), r1 = min(runs.end, r0 + per);
   // the first run's records, on the way while the row's start is put together (mostly there is no other)
   const int any_run = min(r0, g.runs - 1);
   double mass0 = run_mass[any_run];
@@ -1167,7 +1204,7 @@ __device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& s
   }
   int last_col = g.cols;  // of the logits equal to the cut
   if constexpr (!Bins<T>::kExact) {
-    if (inside && !g.open && st.cut.bin >= 0) {
+    if (inside && !g.open && st.cut.inside) {
       cut_inside<T>(g, row, st, &last_col, *inside);
       mass0 = run_mass[any_run];
     }
@@ -1183,7 +1220,7 @@ __device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& s
   if (!all_ties) {
     for (int i = r0; i < r1; ++i) ties += i == r0 ? ties0 : run_ties[i];
     uint32_t all;
-    seen = block_before<uint32_t>(ties, sh.utmp, &all);
+    seen = from.ties + block_before<uint32_t>(ties, sh.utmp, &all);
   }
   auto mass_of = [&](int i, uint32_t& ties_before) {
     const double m = i == r0 ? mass0 : run_mass[i];
@@ -1198,7 +1235,8 @@ __device__ __forceinline__ void pick_row(const SampleArgs& g, int64_t row, S&& s
 #pragma unroll 1
   for (int i = r0; i < r1; ++i) mass += mass_of(i, rank);
   double total;
-  const double before = block_before<double>(mass, sh.dtmp, &total);
+  const double before = from.before + block_before<double>(mass, sh.dtmp, &total);
+  if (from.part >= 0) total = from.total;
   if (!(total > 0.0 && total < INFINITY && max < INFINITY)) {  // (only an open row's can be)
     if (threadIdx.x == 0) g.ids[row] = -1, g.logp[row] = __builtin_nanf("");
     return;
@@ -1390,7 +1428,7 @@ __device__ __forceinline__ void end_listed(const SampleArgs& g, int64_t row, Sta
   st.cut = r.find(sh.cut, st.a, false);
   st.cut_min_p();
   __syncthreads();
-  mass_block<T>(g, row, 0, 1, st, sh.rest.mass);
+  mass_block<T>(g, row, {0, g.runs}, 0, 1, st, sh.rest.mass);
   __syncthreads();
   pick_row<T>(g, row, [&] { return st; }, sh.rest.pick, nullptr);
 }
@@ -1524,6 +1562,10 @@ constexpr int kFlag = 3;  // the place of h.mass that counts what was flagged
 struct CountShared {
   ScanShared scan;
   int first[kWaves];
+  // for choose_part
+  float max;
+  Cut cut;
+  bool counted;  // the counts tell all kept masses
 };
 
 // Counts one block's runs into h. h.mass[1] sums 2^(x k) of |x| < 2^-16.
@@ -1534,8 +1576,9 @@ __device__ __forceinline__ void count_block(Hist<__bf16>& h, const SampleArgs& g
   __syncthreads();
   constexpr int kLow = B::kUsed - 1;
   uint32_t low = 0;
+  const Runs runs = runs_of(g, part);
   each_run(
-      x, g.cols, g.run_cols, g.runs, part * kWaves + (int)threadIdx.x / kWave, g.split * kWaves,
+      x, g.cols, g.run_cols, runs.end, runs.begin + (int)threadIdx.x / kWave, kWaves,
       [&](const Pack<__bf16, 8>& p, int) {
         B::Two least = (B::Two)((short)B::kSide), most = (B::Two)((short)0);
 #pragma unroll
@@ -1562,7 +1605,8 @@ __device__ __forceinline__ void count_block(Hist<__bf16>& h, const SampleArgs& g
   if (threadIdx.x % kWave == 0) atomicAdd(&h.count[kLow], low);
 }
 
-// The row's maximum, sum and cut from the counts of all its columns.
+// The row's maximum, sum and cut from the counts of all its columns. CHOOSES: choose_part comes after it.
+template <bool CHOOSES>
 __device__ __forceinline__ void cut_counted(CutShared<__bf16>& sh, CountShared& own, const SampleArgs& g, int64_t row,
                                             const Asked& a) {
   typedef Bins<__bf16> B;
@@ -1587,6 +1631,7 @@ __device__ __forceinline__ void cut_counted(CutShared<__bf16>& sh, CountShared& 
   if (again) scan_block(x, g, 0, 1, (float)a.k, nullptr, own.scan, &max, &sum);
   const Row<__bf16> r(g, row, a, max);
   const bool ok = !again || (sum > 0.f && sum < INFINITY && max < INFINITY);
+  if (CHOOSES && threadIdx.x == 0) own.max = max, own.counted = !again && a.in_range;
   __syncthreads();
   if (again && ok && cuts) r.fill(sh.hist, 0, 1, a.by_p);
   if (!again && threadIdx.x == 0)  // in terms of the maximum from here on
@@ -1601,7 +1646,10 @@ __device__ __forceinline__ void cut_counted(CutShared<__bf16>& sh, CountShared& 
     g.part_max[row * g.split + threadIdx.x] = threadIdx.x == 0 ? max : -INFINITY;
     g.part_sum[row * g.split + threadIdx.x] = threadIdx.x == 0 ? sum : 0.f;
   }
-  if (threadIdx.x == 0) g.cuts[row] = cut;
+  if (threadIdx.x == 0) {
+    g.cuts[row] = cut;
+    if constexpr (CHOOSES) own.cut = cut;
+  }
 }
 
 template <bool WHOLE>
@@ -1614,7 +1662,7 @@ __global__ __launch_bounds__(kLanes) void sample_count_kernel(SampleArgs g) {
   const __bf16* x = static_cast<const __bf16*>(g.logits) + row * g.ld;
   count_block(sh.hist, g, x, a, part);
   if constexpr (WHOLE) {
-    cut_counted(sh, own, g, row, a);
+    cut_counted<false>(sh, own, g, row, a);
   } else {
     __syncthreads();
     u32x4* to = reinterpret_cast<u32x4*>(static_cast<Hist<__bf16>*>(g.hist) + blockIdx.x);
@@ -1623,11 +1671,86 @@ __global__ __launch_bounds__(kLanes) void sample_count_kernel(SampleArgs g) {
   }
 }
 
+// The part that the token lies in, from the parts' counts: the masses of that part's runs are all that is left to sum
+// (256 rows of 151936 with top-p 0.95: two parts a row, mass 21 us, 34 for whole rows).
+struct ChooseShared {
+  double table[Bins<__bf16>::kUsed];
+  double part[kWaves];
+  uint32_t ties[kMaxSplit];
+};
+__device__ __forceinline__ Chosen choose_part(const SampleArgs& g, int64_t row, const Asked& a, float max, const Cut& cut,
+                                              ChooseShared& sh) {
+  typedef Bins<__bf16> B;
+  Chosen none = {0.0, 0.0, 0, -1};
+  // (a cut among |x| < 2^-16, or below -2^8 and not at -inf, splits a bin)
+  const bool all = cut.x == -INFINITY;
+  if (!all && B::several(B::of(cut.x))) return none;
+  // the bin of |x| < 2^-16, as count_block sums it: with a maximum below it has none, and with one far above it too little
+  // to say which of its logits have any mass
+  const bool zero = cut.x < 0.f && max > 0.f;
+  const double of_zero = zero ? exp2_product(-(double)max, a.k) : 0.0;
+  if (zero && of_zero < 0x1p-1000) return none;
+  const Row<__bf16> r(g, row, a, max);
+  const Hist<__bf16>* from = static_cast<const Hist<__bf16>*>(g.hist) + row * g.split;
+  const bool all_ties = cut.ties >= cut.equal;
+  const int tie_bin = B::of(cut.x);  // (all_ties: not looked at)
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+  const float u = g.u[row];
+#pragma unroll 1
+  for (int b = threadIdx.x; b < B::kUsed; b += kLanes) {
+    const float v = B::value(b);
+    const bool keep = !B::several(b) && v <= max && (all_ties ? v >= cut.x : v > cut.x);
+    sh.table[b] = keep ? r.mass(v) : 0.0;
+  }
+  if (threadIdx.x < g.split && !all_ties) sh.ties[threadIdx.x] = from[threadIdx.x].count[tie_bin];
+  __syncthreads();
+  // several waves a part
+  const int each = kWaves / g.split, part = wave / each, sub = wave % each;
+  double mass = 0.0;
+  if (part < g.split) {
+    const int used = all ? B::kUsed : min(B::kUsed, B::of(cut.x) + 1);
+#pragma unroll 4
+    for (int b = (sub * kWave + lane) * 4; b < used; b += each * kWave * 4) {
+      const u32x4 n = *reinterpret_cast<const u32x4*>(&from[part].count[b]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (b + i < B::kUsed) mass += (double)n[i] * sh.table[b + i];
+    }
+    if (sub == 0 && lane == 0 && zero) mass += (double)from[part].mass[1] / (double)r.fixed(1.0) * of_zero;
+  }
+  mass = wave_total(mass);
+  if (lane == 0) sh.part[wave] = mass;
+  __syncthreads();
+  // (every wave goes through the parts by itself)
+  const double sums = lane < kWaves ? sh.part[lane] : 0.0, one = all_ties ? 0.0 : r.mass(cut.x);
+  const uint32_t equal = lane < g.split && !all_ties ? sh.ties[lane] : 0;
+  Chosen c = none;
+  const double total = wave_total(sums) + (all_ties ? 0.0 : one * (double)cut.ties);
+  uint32_t ties = 0;
+  double before = 0.0;
+#pragma unroll 1
+  for (int p = 0; p < g.split; ++p) {
+    const uint32_t n = of_lane(equal, p), left = cut.ties - min(cut.ties, ties);
+    double m = all_ties ? 0.0 : one * (double)min(left, n);
+    for (int i = 0; i < each; ++i) m += of_lane(sums, p * each + i);
+    if (m > 0.0) c = {before, total, ties, p};
+    ties += n;
+    before += m;
+    if (m > 0.0 && before > (double)u * total) break;
+  }
+  return c;
+}
+
 // (split > 1)
 __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) {
   typedef Bins<__bf16> B;
-  __shared__ __align__(16) CutShared<__bf16> sh;
+  __shared__ union __align__(16) All {
+    CutShared<__bf16> cut;
+    ChooseShared choose;
+    __device__ All() {}
+  } all;
   __shared__ CountShared own;
+  CutShared<__bf16>& sh = all.cut;
   const int64_t row = blockIdx.x;
   const Hist<__bf16>* from = static_cast<const Hist<__bf16>*>(g.hist) + row * g.split;
   const Asked a = asked(g, row);
@@ -1637,7 +1760,16 @@ __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) 
         sum_parts<u32x4>((const char*)&from->count[i], sizeof(Hist<__bf16>), g.split);
   if (threadIdx.x < B::kMasses) sh.hist.mass[threadIdx.x] =
       sum_parts<u64>((const char*)&from->mass[threadIdx.x], sizeof(Hist<__bf16>), g.split);
-  cut_counted(sh, own, g, row, a);
+  cut_counted<true>(sh, own, g, row, a);
+  __syncthreads();
+  Chosen c = {0.0, 0.0, 0, -1};
+  if (g.chosen && own.counted) {
+    Cut cut = own.cut;
+    const Asked again = asked(g, row);  // (not kept in registers over all this)
+    apply_min_p(cut, again, own.max);
+    c = choose_part(g, row, again, own.max, cut, all.choose);
+  }
+  if (g.chosen && threadIdx.x == 0) g.chosen[row] = c;
 }
 
 // How a call is cut up. Two blocks a CU, so want = 2 CUs / rows blocks a row; runs as long as they can be (each costs a
@@ -1658,7 +1790,7 @@ Shape shape_of(int64_t rows, int64_t cols, int64_t cus) {
 }
 
 struct Layout {
-  size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, run_ref, hist, cuts, list, listed, total;
+  size_t part_max, part_sum, quarters, run_mass, run_ties, run_max, run_ref, hist, cuts, chosen, list, listed, total;
 };
 Layout layout_of(int64_t rows, int64_t cols, const Shape& shape, bool cuts, bool bf16) {
   const int64_t runs = shape.runs, split = shape.split;
@@ -1682,6 +1814,7 @@ Layout layout_of(int64_t rows, int64_t cols, const Shape& shape, bool cuts, bool
       l.list = take((size_t)(rows * split) * kPartList * sizeof(Listed));
       l.listed = take((size_t)(rows * split) * sizeof(uint32_t));
     }
+    if (split > 1 && bf16 && runs * shape.run_cols >= split * kChooseCols) l.chosen = take((size_t)rows * sizeof(Chosen));
     if (split > 1) l.hist = take((size_t)(rows * split) * (bf16 ? sizeof(Hist<__bf16>) : sizeof(Hist<float>)));
   }
   l.total = at;
@@ -1766,6 +1899,8 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   // the counts or lists that the row's own k asks for.
   g.lists = cols >= kListCols && !(top_k_rows && dtype == kBF16);
   const bool all_listed = g.lists && !top_k_rows && top_k > 0 && top_k < cols && top_k <= list_most(g.runs);
+  if (cuts && !all_listed && split > 1 && dtype == kBF16 && shape.runs * shape.run_cols >= split * kChooseCols)
+    g.chosen = (Chosen*)(ws + l.chosen);
   const hipStream_t st = (hipStream_t)stream;
   const dim3 parts((unsigned)(rows * split)), each((unsigned)rows);
   const auto run = [&](void (*kernel)(SampleArgs), const dim3& grid, const char* name) {

@@ -40,7 +40,7 @@ def hilda_sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
     among equal ones), of these the shortest prefix in descending order whose probability reaches ``top_p`` of theirs
     (>= 1: all), of these the tokens with at least ``min_p`` times the largest probability. The id is the first kept
     token, by index, whose cumulative probability exceeds ``uniform``. logp is its log_softmax(logits / temperature)
-    over all tokens, as ``fused_selective_log_softmax`` gives it.
+    over all tokens, as ``fused_selective_log_softmax`` gives it. Neither carries a gradient.
 
     A row that holds a NaN or +inf or nothing above -inf, or whose own temperature, uniform number or setting is NaN
     or out of range, gives id -1 and logp NaN.

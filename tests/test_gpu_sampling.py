@@ -385,3 +385,35 @@ def test_cuts_among_masked_tokens(dtype):
     x[6] = x[6].abs() * 200
     for kw in (dict(top_k=400), dict(top_k=8999), dict(top_p=0.999), dict(top_k=500, top_p=0.99), dict(top_k=1000, min_p=0.5)):
         _check(x, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [40009, 151936])
+def test_parts_of_a_row(dtype, V):
+    """Rows that several blocks share: draws at both ends of each share, shares without mass, ties over all of them."""
+    rows = 30
+    x, u, g = _rows(rows, V, dtype, seed=V + 1, lo=0.5, hi=5.0)
+    x[0] = 0.0
+    x[1, : V // 3] = -math.inf
+    x[2, V // 5:] = -math.inf
+    x[3, V // 5: -V // 5] = torch.finfo(dtype).min
+    x[4] = torch.where(torch.rand(V, generator=g) < 0.5, 1.5, -20.0).to(dtype)
+    x[5] = (x[5].float() * 1e-6).to(dtype)
+    x[6] = (x[6].float() * 200).clamp(-6e4, 6e4).to(dtype)
+    x[7] = -x[7].abs() - 3
+    x[8, ::2] = 0.0
+    x[9] = -math.inf
+    x[9, -1] = 3.0
+    x[10, V // 2] = math.nan
+    u[11], u[12], u[13], u[14] = 0.0, 1.0, 1 - 2.0 ** -24, 0.5
+    u[1], u[2], u[9] = 0.0, 1.0, 1.0
+    for kw in (dict(top_p=0.95), dict(top_p=0.6, min_p=0.01), dict(top_k=1000), dict(top_k=V // 2, temperature=0.7),
+               dict(top_k=5000, top_p=0.9), dict(top_p=0.5, temperature=0.05)):
+        _check(x, u, **kw)
+        _check(x, u.flip(0), **kw)
+    _check(x, u, top_k=torch.randint(-5, 3000, (rows,), generator=g), top_p=0.5 + torch.rand(rows, generator=g),
+           min_p=0.01 * torch.rand(rows, generator=g), temperature=0.5 + torch.rand(rows, generator=g))
+    # one row over many blocks, from end to end
+    for v in torch.linspace(0, 1, 41).tolist():
+        _check(x[14:15], torch.tensor([v]), top_p=0.9)
+        _check(x[4:5], torch.tensor([v]), top_k=V // 3)
