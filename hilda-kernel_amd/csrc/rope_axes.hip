@@ -198,8 +198,9 @@ int hk_rope_axes(void* q_out, const void* q_in, void* k_out, const void* k_in, c
   const int64_t half = D / 2;
   RopeAxesArgs g = {};
   int64_t sum = 0;
+  for (int a = 0; a < axes; ++a) HK_REQUIRE(sections[a] >= 0, "sections must not be negative");
   for (int a = 0; a < axes; ++a) {
-    HK_REQUIRE(sections[a] >= 0, "sections must not be negative");
+    HK_REQUIRE(sections[a] <= half, "section %d has %lld pairs of D/2 = %lld", a, (long long)sections[a], (long long)half);
     sum += sections[a];
     g.axes.n[a] = (int)(shape->interleaved ? sections[a] : sum);
   }

@@ -417,3 +417,80 @@ def test_parts_of_a_row(dtype, V):
     for v in torch.linspace(0, 1, 41).tolist():
         _check(x[14:15], torch.tensor([v]), top_p=0.9)
         _check(x[4:5], torch.tensor([v]), top_k=V // 3)
+
+
+# every chain of launches: no filter, min-p alone, lists, bins (one filter, two, parts that are chosen), a value each
+CHAINS = [(1, 9001, dict()), (3, 9001, dict(min_p=0.1)), (1, 30011, dict(top_k=40)), (300, 9001, dict(top_k=40, top_p=0.9)),
+          (2, 30011, dict(top_p=0.9)), (300, 9001, dict(top_p=0.9)), (2, 30011, dict(top_k=900, top_p=0.9)),
+          (200, 80011, dict(top_p=0.95, min_p=1e-4)), (40, 30011, "each"), (300, 9001, "each")]
+
+
+def _chain(case, dtype, seed):
+    rows, V, kw = case
+    x, u, g = _rows(rows, V, dtype, seed=seed)
+    if kw == "each":
+        kw = dict(temperature=0.5 + torch.rand(rows, generator=g), top_k=torch.randint(-50, 400, (rows,), generator=g),
+                  top_p=0.6 + 0.5 * torch.rand(rows, generator=g), min_p=0.01 * torch.rand(rows, generator=g))
+    dev = gpu()
+    return [x.to(dev), u.to(dev)], {k: v.to(dev) if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", CHAINS, ids=lambda c: f"{c[0]}x{c[1]}-{c[2] if c[2] == 'each' else '-'.join(c[2])}")
+def test_repeats_graphs_and_used_workspaces(dtype, case):
+    """The same numbers on every call, in a captured graph with new logits, and whatever the workspace held before."""
+    (x, u), kw = _chain(case, dtype, 40)
+    (x2, u2), kw2 = _chain(case, dtype, 41)
+    first, other = hilda_sample(x, u, **kw), hilda_sample(x2, u2, **kw2)
+    for fill in (0, 255, 127):
+        junk = torch.full((64 << 20,), fill, dtype=torch.uint8, device=gpu())
+        del junk  # the next workspace is cut from it
+        again = hilda_sample(x, u, **kw)
+        assert torch.equal(again[0], first[0]) and torch.equal(again[1], first[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        hilda_sample(x, u, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = hilda_sample(x, u, **kw)
+    held = [t.clone() for t in (x, u)], {k: v.clone() for k, v in kw.items() if isinstance(v, torch.Tensor)}
+    for n in range(4):
+        src, want = ((x2, u2), kw2), other
+        if n % 2:
+            src, want = held, first
+        x.copy_(src[0][0])
+        u.copy_(src[0][1])
+        for k, v in kw.items():
+            if isinstance(v, torch.Tensor):
+                v.copy_(src[1][k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]), f"replay {n}"
+
+
+@pytest.mark.parametrize("kw", [dict(top_p=0.95), dict(top_k=2000, min_p=1e-3), "each"], ids=["p", "km", "each"])
+def test_few_long_parts(kw):
+    """As test_parts_of_a_row, with so many rows that two blocks share one: the token's part is told by the counts."""
+    V, rows = 75011, 240
+    x, _, g = _rows(24, V, torch.bfloat16, seed=50, lo=0.5, hi=5.0)
+    x[0] = 0.0
+    x[1, : V // 3] = -math.inf
+    x[2, V // 5:] = -math.inf
+    x[3, 100: V // 2] = torch.finfo(torch.bfloat16).min
+    x[4] = torch.where(torch.rand(V, generator=g) < 0.5, 1.5, -20.0).to(torch.bfloat16)
+    x[5] = (x[5].float() * 1e-6).to(torch.bfloat16)
+    x[6] = (x[6].float() * 200).to(torch.bfloat16)
+    x[7] = -x[7].abs() - 3
+    x[8, ::2], x[8, 5::8] = 0.0, 2.0 ** -30
+    x[9] = -math.inf
+    x[9, -1] = 3.0
+    x[10, V // 2] = math.nan
+    x = x.repeat(rows // 24, 1)
+    u = torch.rand(rows, generator=g)
+    u[:24], u[24:48], u[48:72], u[72:96] = 0.0, 1.0, 1 - 2.0 ** -24, 0.5
+    if kw == "each":
+        kw = dict(top_k=torch.randint(-9000, 9000, (rows,), generator=g), top_p=0.5 + torch.rand(rows, generator=g),
+                  min_p=0.01 * torch.rand(rows, generator=g), temperature=0.05 + torch.rand(rows, generator=g))
+    _check(x, u, **kw)

@@ -139,6 +139,8 @@ def test_rope_axes_refusals():
     _einval(call(sections=(70, -3, -3)), "negative")
     _einval(call(axes=5), "axes")
     _einval(call(axes=0), "axes")
+    # (their sum passes 64 bits and comes to 64)
+    _einval(call(sections=(1 << 62, 1 << 62, 1 << 62, (1 << 62) + 64)), "pairs of")
     # axis 1 of 2 over 64 pairs owns at most 32
     _einval(call(sections=(30, 34), interleaved=1), "interleaved section")
     _einval(call(sections=(0, 32, 32), interleaved=1), "interleaved section")
