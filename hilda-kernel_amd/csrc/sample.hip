@@ -28,7 +28,8 @@
 //   list   the few logits at or above a bound on the k-th, taken from the scan's
 //          maxima, and (draw) the token from them, ordered. One reading of the
 //          row and two launches less than bins: 256 rows of 151936 fp32 logits
-//          with k = 50 take 65 us, 124 by bins; one bf16 row of 128256 20 us, 30.
+//          with k = 50 take 65 us, with k = 209 by bins 99; one bf16 row of 128256
+//          20 and 31.
 //   hist   counts, and for top-p masses, in bins linear in max - x
 //   count  counts in bins of one bf16 value each, which give the maximum, the
 //          sum and every mass
@@ -39,7 +40,7 @@
 //          logits or less and there is one filter, mass lists them and pick finds
 //          the cut in their order instead: a block takes 25 to 45 us to read a
 //          row of 151936 fp32 logits, mass reads them anyway, and pick takes 10 us
-//          more (256 such rows with top-p: 176 us, 193 before).
+//          more (256 such rows with top-p: 174 us, 193 before).
 //          Of bf16 rows in few long parts it also tells the part that the
 //          token lies in, by the parts' counts.
 //   mass   the kept mass of each run (of that part)

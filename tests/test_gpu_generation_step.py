@@ -147,3 +147,42 @@ def test_other_streams_and_two_threads():
     for a, b in zip(got, want):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+def test_elements_beyond_32_bit_offsets():
+    """More than 2^31 elements a tensor: the last rows come out as they do alone."""
+    dev, bf = gpu(), torch.bfloat16
+    g = torch.Generator(device=dev).manual_seed(6)
+
+    rows, hidden, n = 530_000, 4096, 5
+    x = torch.zeros(rows, hidden, device=dev, dtype=bf)
+    x[-n:] = torch.randn(n, hidden, device=dev, generator=g).to(bf)
+    w = torch.randn(hidden, device=dev, generator=g).to(bf)
+    assert x.numel() > 2 ** 31
+    whole = K.hilda_fused_add_rms_norm_quant(x, x, w, group_size=128)
+    alone = K.hilda_fused_add_rms_norm_quant(x[-n:], x[-n:], w, group_size=128)
+    for a, b in zip(whole, alone):
+        assert torch.equal(a[-n:].view(torch.uint8), b.view(torch.uint8))
+    del x, whole
+
+    T = 4_200_000
+    q = torch.zeros(1, T, 4, 128, device=dev, dtype=bf).transpose(1, 2)
+    k = torch.randn(1, T, 1, 128, device=dev, generator=g).to(bf).transpose(1, 2)
+    q[:, :, -n:] = torch.randn(1, 4, n, 128, device=dev, generator=g).to(bf)
+    rot = K.MultiAxisRotaryEmbedding(128, (16, 24, 24), 512).to(dev)
+    pos = torch.randint(0, 512, (3, 1, T), device=dev, generator=g)
+    assert q.numel() > 2 ** 31
+    whole, alone = rot(q, k, pos), rot(q[:, :, -n:], k[:, :, -n:], pos[:, :, -n:])
+    for a, b in zip(whole, alone):
+        assert torch.equal(a[:, :, -n:], b)
+    del q, k, whole
+
+    rows, vocab = 14_200, 151936
+    x = torch.zeros(rows, vocab, device=dev, dtype=bf)
+    x[-n:] = (3 * torch.randn(n, vocab, device=dev, generator=g)).to(bf)
+    u = torch.rand(rows, device=dev, generator=g)
+    assert x.numel() > 2 ** 31
+    for kw in ({}, dict(top_k=50), dict(top_p=0.9), dict(min_p=0.01)):
+        whole, alone = K.hilda_sample(x, u, **kw), K.hilda_sample(x[-n:], u[-n:], **kw)
+        assert torch.equal(whole[0][-n:], alone[0])
+        assert torch.allclose(whole[1][-n:], alone[1], rtol=1e-5, atol=1e-5)
