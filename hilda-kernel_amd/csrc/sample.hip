@@ -49,7 +49,7 @@
 // What bounds it: the first pass of 256 rows of 151936 bf16 logits (78 MB) runs
 // at HBM's rate (scan 15 us); the bins' LDS atomics (count 23 us) and the mass
 // table's LDS gathers (mass 21 us, 33 cycles a wave's) are LDS-bound, cut, draw
-// and pick (16, 7 and 8 us) chains of latencies. 69 us in all with top-p, 35
+// and pick (17, 7 and 8 us) chains of latencies. 69 us in all with top-p, 33
 // without filters; few rows are bound by those chains, 4 to 14 us a launch. fp32
 // and fp16 pay for e^(z - max) in fp64 in hist and mass (50 and 57 us with top-p).
 //
@@ -75,7 +75,7 @@ typedef unsigned long long u64;
 
 constexpr int kLanes = 1024;          // threads of a block
 constexpr int kWaves = kLanes / kWave;
-constexpr int kMaxSplit = 16;         // blocks a row
+constexpr int kMaxSplit = 16;         // blocks a row at most
 constexpr int kFineBins = 2048;
 // the linear bins cover max - x < kRange * T; beyond it is one bin
 constexpr double kRange = 24;
@@ -1773,18 +1773,24 @@ __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) 
   if (g.chosen && threadIdx.x == 0) g.chosen[row] = c;
 }
 
-// How a call is cut up. Two blocks a CU, so want = 2 CUs / rows blocks a row; runs as long as they can be (each costs a
-// sum over the wave) while there are four for every wave, so that no wave has much more than another; and of the blocks
-// that need the same number of turns, the fewest.
+// How a call is cut up. One block a CU, so want = CUs / rows blocks a row (two a CU have more bins to put together and a
+// cut of their own to launch; us with one and two: 64 x 151936 bf16 top-p 42 and 46, min-p 22 and 26; 256 rows top-k 5000
+// 55 and 63, no filter 33 and 36; fp32 61 and 65, 24 and 25, 125 and 129, 61 and 60), but two a CU for fp32 and fp16
+// without top-k and top-p, whose fp64 exponentials need the waves (256 rows with min-p 0.02 87 and 72); and two blocks a
+// row to choose from for bf16 rows that top-p alone cuts (256 rows 70 and 75 us, 300 rows 102 and 117, 600 rows the same). Runs as long as they
+// can be (each costs a sum over the wave) while there are eight for every wave, so that no wave has much more than
+// another; and of the blocks that need the same number of turns, the fewest.
 struct Shape {
   int64_t run_cols, runs, split;
 };
-Shape shape_of(int64_t rows, int64_t cols, int64_t cus) {
+Shape shape_of(int64_t rows, int64_t cols, int64_t cus, bool cuts, bool bf16, bool chooses) {
   Shape s;
   s.run_cols = 2048;
   while (s.run_cols > 512 && rows * cdiv(cols, s.run_cols) < 8 * cus * kWaves) s.run_cols /= 2;
   s.runs = cdiv(cols, s.run_cols);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, 2 * cus / std::max<int64_t>(rows, 1)));
+  const int64_t blocks = cuts || bf16 ? cus : 2 * cus;
+  int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxSplit, blocks / std::max<int64_t>(rows, 1)));
+  if (chooses && bf16 && want == 1 && rows <= 2 * cus && cols >= 2 * kChooseCols) want = 2;
   const int64_t turns = cdiv(s.runs, want * kWaves);
   s.split = cdiv(s.runs, turns * kWaves);
   return s;
@@ -1831,8 +1837,12 @@ extern "C" {
 
 size_t hk_sample_workspace_size(int64_t rows, int64_t cols, int cuts, int dtype, int device) {
   if (rows < 0 || rows >= (1LL << 31) || cols <= 0 || cols > (1 << 30)) return 0;
-  const int cus = cu_count(device);
-  return std::max<size_t>(256, layout_of(rows, cols, shape_of(rows, cols, cus > 0 ? cus : 256), cuts != 0, dtype == kBF16).total);
+  const int cus = cu_count(device) > 0 ? cu_count(device) : 256;
+  size_t most = 256;
+  for (const bool chooses : {false, true})
+    most = std::max(most, layout_of(rows, cols, shape_of(rows, cols, cus, cuts != 0, dtype == kBF16, chooses), cuts != 0,
+                                    dtype == kBF16).total);
+  return most;
 }
 
 int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int64_t rows, int64_t cols, int64_t ld,
@@ -1856,10 +1866,11 @@ int hk_sample(int64_t* ids, float* logp, const void* logits, const float* u, int
   const int dev = current_device();
   if (dev < 0) return (int)hipErrorNoDevice;
   const int cus = cu_count(dev);
-  const Shape shape = shape_of(rows, cols, cus > 0 ? cus : 256);
+  const bool cuts = top_k_rows || (top_k > 0 && top_k < cols) || top_p_rows || top_p < 1;
+  const bool by_mass = (top_p_rows || top_p < 1) && !top_k_rows && !(top_k > 0 && top_k < cols);
+  const Shape shape = shape_of(rows, cols, cus > 0 ? cus : 256, cuts, dtype == kBF16, by_mass);
   const int split = (int)shape.split;
   HK_REQUIRE(rows * split < (1LL << 32) / kLanes, "rows=%lld too many for one launch", (long long)rows);
-  const bool cuts = top_k_rows || (top_k > 0 && top_k < cols) || top_p_rows || top_p < 1;
   const bool masses = cuts || min_p_rows || min_p > 0;
   const Layout l = layout_of(rows, cols, shape, cuts, dtype == kBF16);
   HK_REQUIRE(workspace_bytes >= l.total, "workspace too small: need %zu bytes, got %zu", l.total, workspace_bytes);
