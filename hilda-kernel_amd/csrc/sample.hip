@@ -36,7 +36,7 @@
 //   cut    the bins of a row's blocks together; the bin that holds the cut; if
 //          several values may lie in it, the same over ranges of ordered keys,
 //          11 bits at a time, until one is left: x* and how many ties are kept.
-//          With one block a row this ends the launch before. If the bin has 512
+//          With one block a row this ends the launch before. If the bin has 768
 //          logits or less and there is one filter, mass lists them and pick finds
 //          the cut in their order instead: a block takes 25 to 45 us to read a
 //          row of 151936 fp32 logits, mass reads them anyway, and pick takes 10 us
@@ -82,16 +82,18 @@ constexpr double kRange = 24;
 constexpr double kTempMin = 0x1p-64, kTempMax = 0x1p64;
 constexpr double kLog2eD = 1.4426950408889634074, kLn2D = 0.69314718055994530942;
 constexpr int kGroups = 256;          // maxima that a bound on the k-th logit is taken from
-// Columns of a part at least for a choice of the part (choose_part takes 6 us; bf16, top-p 0.95 and 0.5, with and without:
-// 256 rows in parts of 76000 71 and 81, 61 and 61 us; 128 of 38000 52 and 56, 48 and 47; 256 of 33000 51 and 53, 48 and 45;
-// 1 of 8000 39 and 33, 37 and 31).
-constexpr int64_t kChooseCols = 36 << 10;
+// Columns of a part at least for a choice of the part (choose_part takes 4 to 6 us; bf16, top-p 0.95 and top-k 5000, with
+// and without: 128 rows in parts of 76000 52 and 55, 46 and 45 us; 100 of 50000 45 and 45, 42 and 39; 64 of 38000 43 and
+// 43, 42 and 38).
+constexpr int64_t kChooseCols = 64 << 10;
 // Rows of few kept logits go by a list of those at or above that bound: for k = 208 of 256 groups it has about
-// 256 ln(256 / 48) = 430 of them, for k = 50 some 56. (64 x 151936 bf16: k = 20 25 us, 208 37; by bins k = 209 40.)
+// 256 ln(256 / 48) = 430 of them, for k = 50 some 56. (64 x 151936 bf16: k = 20 23 us, 208 38; by bins k = 209 39.
+// 256 x 151936 fp32: 66, 81; 97.)
 constexpr int kListMost = 208;        // k of such a row at most
-constexpr int kPartList = 512, kList = 768;  // room for a block's, and a row's
-// columns at least: the lists then have half the bytes of the logits at most. 512 rows of 8192 with k = 50 take 27 us,
-// by bins 40 (bf16) and 47 (fp32).
+// (430 has a deviation of 26; a list short of room costs three more readings of the row.)
+constexpr int kPartList = 768, kList = 768;  // room for a block's, and a row's
+// columns at least: the lists then have three quarters of the logits' bytes at most. 512 rows of 8192 with k = 50 take 26
+// us, by bins 44.
 constexpr int kListCols = 8192;
 __host__ __device__ constexpr int list_most(int runs) { return 4 * runs < kListMost ? 4 * runs : kListMost; }
 
@@ -1764,7 +1766,8 @@ __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) 
   cut_counted<true>(sh, own, g, row, a);
   __syncthreads();
   Chosen c = {0.0, 0.0, 0, -1};
-  if (g.chosen && own.counted) {
+  // (if fewer are kept than a wave's 512 logits hold one of, their masses cost less than the choice)
+  if (g.chosen && own.counted && own.cut.count > (uint32_t)g.cols / 512) {
     Cut cut = own.cut;
     const Asked again = asked(g, row);  // (not kept in registers over all this)
     apply_min_p(cut, again, own.max);
@@ -1777,7 +1780,8 @@ __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) 
 // cut of their own to launch; us with one and two: 64 x 151936 bf16 top-p 42 and 46, min-p 22 and 26; 256 rows top-k 5000
 // 55 and 63, no filter 33 and 36; fp32 61 and 65, 24 and 25, 125 and 129, 61 and 60), but two a CU for fp32 and fp16
 // without top-k and top-p, whose fp64 exponentials need the waves (256 rows with min-p 0.02 87 and 72); and two blocks a
-// row to choose from for bf16 rows that top-p alone cuts (256 rows 70 and 75 us, 300 rows 102 and 117, 600 rows the same). Runs as long as they
+// row to choose from for bf16 rows that top-p alone cuts (256 rows with 0.95 70 and 75 us, 0.5 60 and 52; 300 rows 102 and 118, 88 and 88; 600
+// rows the same). Runs as long as they
 // can be (each costs a sum over the wave) while there are eight for every wave, so that no wave has much more than
 // another; and of the blocks that need the same number of turns, the fewest.
 struct Shape {

@@ -422,7 +422,7 @@ def test_parts_of_a_row(dtype, V):
 # every chain of launches: no filter, min-p alone, lists, bins (one filter, two, parts that are chosen), a value each
 CHAINS = [(1, 9001, dict()), (3, 9001, dict(min_p=0.1)), (1, 30011, dict(top_k=40)), (300, 9001, dict(top_k=40, top_p=0.9)),
           (2, 30011, dict(top_p=0.9)), (300, 9001, dict(top_p=0.9)), (2, 30011, dict(top_k=900, top_p=0.9)),
-          (200, 80011, dict(top_p=0.95, min_p=1e-4)), (40, 30011, "each"), (300, 9001, "each")]
+          (100, 140011, dict(top_p=0.95, min_p=1e-4)), (40, 30011, "each"), (300, 9001, "each")]
 
 
 def _chain(case, dtype, seed):
@@ -473,7 +473,7 @@ def test_repeats_graphs_and_used_workspaces(dtype, case):
 @pytest.mark.parametrize("kw", [dict(top_p=0.95), dict(top_k=2000, min_p=1e-3), "each"], ids=["p", "km", "each"])
 def test_few_long_parts(kw):
     """As test_parts_of_a_row, with so many rows that two blocks share one: the token's part is told by the counts."""
-    V, rows = 75011, 240
+    V, rows = 140011, 120
     x, _, g = _rows(24, V, torch.bfloat16, seed=50, lo=0.5, hi=5.0)
     x[0] = 0.0
     x[1, : V // 3] = -math.inf
