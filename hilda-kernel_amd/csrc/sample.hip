@@ -1780,10 +1780,10 @@ __global__ __launch_bounds__(kLanes) void sample_count_cut_kernel(SampleArgs g) 
 // cut of their own to launch; us with one and two: 64 x 151936 bf16 top-p 42 and 46, min-p 22 and 26; 256 rows top-k 5000
 // 55 and 63, no filter 33 and 36; fp32 61 and 65, 24 and 25, 125 and 129, 61 and 60), but two a CU for fp32 and fp16
 // without top-k and top-p, whose fp64 exponentials need the waves (256 rows with min-p 0.02 87 and 72); and two blocks a
-// row to choose from for bf16 rows that top-p alone cuts (256 rows with 0.95 70 and 75 us, 0.5 60 and 52; 300 rows 102 and 118, 88 and 88; 600
-// rows the same). Runs as long as they
-// can be (each costs a sum over the wave) while there are eight for every wave, so that no wave has much more than
-// another; and of the blocks that need the same number of turns, the fewest.
+// row to choose from for bf16 rows that top-p alone cuts (256 rows with 0.95 70 and 75 us, with 0.5 60 and 52; 300 rows 102
+// and 118, 88 and 88; 600 rows the same). Runs as long as they can be (each costs a sum over the wave) while there are
+// eight for every wave, so that no wave has much more than another; and of the blocks that need the same number of turns,
+// the fewest.
 struct Shape {
   int64_t run_cols, runs, split;
 };
